@@ -14,6 +14,7 @@
  *                       surgery addToOptimizer / removeFromOptimizer, model.cpp:253-309: builds the
  *                       six parameter tensors and their twelve Adam moment tensors of the new set
  *   gs_reset_opacity    the "alpha reset", model.cpp:464-479
+ * and, beside them, the fixed-budget strategy the reference lacks: gs_sample, gs_relocate.
  *
  * Element order of the new set = the reference's: cat({originals, split samples (sample-major:
  * repeat({nSplitSamples, 1})), duplicates}) followed by index({~culls}).
@@ -107,6 +108,64 @@ int gs_densify_apply(int N, int K, int new_N /* counts[GS_DENSIFY_NEW_N] */, con
  * installs it, model.cpp:475-477 — pass NULL moments to reproduce exactly that.) */
 int gs_reset_opacity(int N, float reset_value, float *opacity_logits, float *exp_avg,
                      float *exp_avg_sq, gs_stream_t stream);
+
+/* ---- a fixed budget of Gaussians: draw sources, relocate the dead onto them --------------------------------------
+ * (The reference densifies by gradient thresholds only.  This is the other strategy in use: the number of Gaussians is
+ * given, and those that have become transparent move to where sources drawn by their opacity are.) */
+
+enum { GS_DTYPE_F32 = 0, GS_DTYPE_F16 = 1, GS_DTYPE_BF16 = 2 };
+
+/* How gs_sample weighs a row.  The four scalars hold for all rows; a non-NULL device array [rows] replaces its scalar.
+ *   temperature  weights are exp((l - max l) / temperature); 0: the first of the order alone (largest, lowest index)
+ *   top_k        <= 0: all candidates
+ *   top_p        >= 1: all;  <= 0: the first alone
+ *   min_p        entries whose weight, relative to the row's largest, is below it are dropped; <= 0: none; the first of
+ *                the order always stays
+ *   flags        GS_FLAG_LOGIT_OPACITY: l = log sigmoid(x), so that at temperature 1 the weights are the opacities;
+ *                otherwise l = x
+ * Scalars out of range (negative or NaN temperature, NaN, min_p > 1) are refused; a row whose array holds a negative or
+ * NaN temperature, or a NaN, draws -1. */
+typedef struct GsSampleConfig {
+    int32_t dtype; /* GS_DTYPE_*: of the logits */
+    uint32_t flags;
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+    const float *temperature_rows; /* device [rows], nullable */
+    const int32_t *top_k_rows;
+    const float *top_p_rows, *min_p_rows;
+} GsSampleConfig;
+
+size_t gs_sample_workspace_bytes(int rows, int cols);
+
+/* ids[r, j]: an index of row r drawn with the given uniforms[r, j] in [0, 1) (values outside are clamped).
+ *   candidates  entries that are not NaN and not -inf; order: descending value, equal values by ascending index
+ *   kept        the first top_k candidates; of these the shortest prefix (one at least) whose weights sum to top_p times
+ *               theirs; of these the ones that reach min_p
+ *   ids[r, j]   the lowest kept index i with  sum of kept weights up to and including i  >  uniforms[r, j] * their sum;
+ *               -1 for a row without candidates and for a NaN uniform
+ * logits [rows, cols] of `dtype`, row r at row_stride elements behind row r - 1 (row_stride >= cols; any alignment of the
+ * element); uniforms and ids [rows, draws] contiguous.  Weights and sums are 64-bit in a fixed order (a weight below the
+ * range of 64 bits is 0 and never drawn): equal calls give equal ids.  No host synchronisation; the workspace (16-byte aligned) may be reused behind the call in stream order. */
+int gs_sample(int rows, int cols, const void *logits, int64_t row_stride, const GsSampleConfig *cfg /*host*/, int draws,
+              const float *uniforms, int32_t *ids, void *workspace, size_t workspace_bytes, gs_stream_t stream);
+
+size_t gs_relocate_workspace_bytes(int N, int pairs);
+
+/* Pair i makes row targets[i] a copy of row sources[i], in place.  A source with c pairs and its c copies become m = c + 1
+ * Gaussians that together keep its opacity o and extent:  o' = 1 - (1 - o)^(1/m) (not below min_opacity),
+ *   scales' = scales * o / sum_{j=1..m} (-1)^(j-1) C(m, j) o''^j / sqrt(j),   o'' = o' before the bound
+ * (Kheradmand et al., 3D Gaussian Splatting as Markov Chain Monte Carlo, 2024); opacity logits above 16 count as 16.  Means,
+ * quaternions and features are copied; the Adam moments of every row written (copies and sources) become 0.
+ *   params      the six tensors (K bases; features_rest NULL when K == 1)
+ *   exp_avg, exp_avg_sq   nullable, as may be any of their tensors
+ * Pairs that do not hold change nothing: an index outside [0, N) (gs_sample's -1 among them), a target that an earlier
+ * pair names, a source that some pair with both indices in range names as its target.  The result does not depend on
+ * the order in which the device takes the pairs. */
+int gs_relocate(int N, int K, int pairs, const int32_t *targets, const int32_t *sources, float min_opacity,
+                const GsGaussianSet *params /*host*/, const GsGaussianSet *exp_avg /*host, nullable*/,
+                const GsGaussianSet *exp_avg_sq /*host, nullable*/, void *workspace, size_t workspace_bytes,
+                gs_stream_t stream);
 
 #ifdef __cplusplus
 }

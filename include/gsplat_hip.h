@@ -93,11 +93,12 @@ const char *gs_strerror(int status);
 const char *gs_last_hip_error(void); /* thread-local text of the last failing HIP call */
 /* ABI version of THIS header: 10000*major + 100*minor + patch.  Bumped whenever an entry point changes its
  * argument list or an entry point is added (0.3.0: block_masks / tile_bins_rows arguments of round 3; 0.4.0:
- * round 4; 0.4.2 / 0.4.3: gs_bin_strips, gs_bin_speculative, 0.4.4: gs_bin_speculative_zero, round 6).  A consumer
+ * round 4; 0.4.2 / 0.4.3: gs_bin_strips, gs_bin_speculative, 0.4.4: gs_bin_speculative_zero,
+ * round 6; 0.4.5: gs_sample, gs_relocate, gs_tile_balance).  A consumer
  * compiled against another header must refuse the library instead of calling through shifted arguments:
  * opensplat_amd/cabi.py compares gs_version() with this constant when it loads the library, libgsplat_torch.so in
  * front of its first call into it (torch_ops.cpp: current_stream()). */
-#define GS_ABI_VERSION 404
+#define GS_ABI_VERSION 405
 int gs_version(void);                /* == GS_ABI_VERSION of the header the library was built from */
 
 /* ---------------------------------------------------------------------------------------------

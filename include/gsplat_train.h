@@ -53,6 +53,24 @@ int gs_main_loss(int W, int H, const float *rendered, const float *gt, float ssi
                  float grad_scale, float *loss, float *v_rendered, void *workspace,
                  size_t workspace_bytes, gs_stream_t stream);
 
+/* Balance loss of a frame's tile lists with its gradient: a penalty on opacity that sits in crowded tiles (a frame's time
+ * is that of its longest lists).  For the T = tiles of the image, n_t = entries of tile t's list, o_g = opacity of
+ * Gaussian g, S_t = the sum of o_g over list t, M = sum n_t, S = sum S_t:
+ *   loss = scale * T * sum_t (n_t / M) (S_t / S)          (scale when all lists are alike; 0 when M or S is 0)
+ * The counts n_t are constants of the gradient, as they are piecewise constant:
+ *   d loss / d o_g = scale * T / (M S) * (A_g - c_g * sum_t n_t S_t / S),  A_g = sum of n_t over the c_g tiles of g.
+ * Gaussians in no list have gradient 0.
+ *   packed      [N, 12] records and tile_bins [T, 2] of the frame's binning (gsplat_hip.h): list t holds the Gaussians
+ *               whose rectangle overlaps tile t, and o_g is the record's opacity
+ *   loss        float[1];   counts: int32 [T] = n_t, nullable;   v_opacity: [N], nullable (value and counts only)
+ *   flags       GS_FLAG_LOGIT_OPACITY: v_opacity is the gradient w.r.t. the opacity logit (times o (1 - o));
+ *               GS_FLAG_ACCUMULATE_GRADS: added to v_opacity (next to gs_gaussian_backward's) instead of written
+ * Sums are 64-bit in a fixed order: equal calls give equal bits. */
+size_t gs_tile_balance_workspace_bytes(int W, int H);
+int gs_tile_balance(int W, int H, int N, const float *packed, const int32_t *tile_bins, float scale, float *loss,
+                    int32_t *counts, float *v_opacity, uint32_t flags, void *workspace, size_t workspace_bytes,
+                    gs_stream_t stream);
+
 /* One parameter group of the optimiser: Model's means / scales / quats / featuresDc /
  * featuresRest / opacities (model.cpp:61-66), each with its own learning rate. */
 typedef struct GsAdamGroup {

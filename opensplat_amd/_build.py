@@ -19,6 +19,8 @@ INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["gs_api.hip", "gs_project.hip", "gs_sh.hip", "gs_bin.hip", "gs_raster.hip",
                "gs_loss.hip", "gs_adam.hip", "gs_densify.hip", "gs_fused.hip", "gs_compat.hip"]
+# compiled on their own, without the packed fp32 instructions the compiler forms from ordinary float code
+HIP_SOURCES_PLAIN = ["gs_sample.hip", "gs_relocate.hip", "gs_balance.hip"]
 HIP_HEADERS = ["gs_device.h", "gs_gaussian.h", os.path.join(INCLUDE, "gsplat_hip.h"),
                os.path.join(INCLUDE, "gsplat_train.h"), os.path.join(INCLUDE, "gsplat_densify.h"),
                os.path.join(INCLUDE, "gsplat_compat.h")]
@@ -32,6 +34,7 @@ TORCH_LIB = os.path.join(CSRC, "libgsplat_torch.so")
 # 386 -> 381 us, k_gaussian_backward 71 -> 67 us at C2, profiles/bench_va_*.json)
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
                "-ffp-contract=off", "-fno-slp-vectorize", "-Wall", "-Wno-unused-function"]
+HIPCC_PLAIN_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target: str, sources: list[str]) -> bool:
@@ -47,11 +50,16 @@ def _run(cmd: list[str]) -> None:
 
 
 def build_hip(force: bool = False) -> str:
-    srcs = [os.path.join(CSRC, s) for s in HIP_SOURCES]
+    srcs = [os.path.join(CSRC, s) for s in HIP_SOURCES + HIP_SOURCES_PLAIN]
     deps = srcs + [h if os.path.isabs(h) else os.path.join(CSRC, h) for h in HIP_HEADERS]
     if force or _stale(HIP_LIB, deps):
         hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-        _run([hipcc] + HIPCC_FLAGS + HIP_SOURCES + ["-o", HIP_LIB])
+        objects = []
+        for s in HIP_SOURCES_PLAIN:
+            objects.append(s.replace(".hip", ".o"))
+            flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+            _run([hipcc] + flags + HIPCC_PLAIN_FLAGS + ["-c", s, "-o", objects[-1]])
+        _run([hipcc] + HIPCC_FLAGS + HIP_SOURCES + objects + ["-o", HIP_LIB])
     return HIP_LIB
 
 

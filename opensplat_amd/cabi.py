@@ -18,7 +18,7 @@ from . import _build
 
 GS_TILE = 16
 GS_SPLAT_DWORDS = 12
-GS_ABI_VERSION = 404   # include/gsplat_hip.h
+GS_ABI_VERSION = 405   # include/gsplat_hip.h
 GS_FLAG_FAST_EXP = 1
 GS_FLAG_LOGIT_OPACITY = 2
 GS_FLAG_CLAMP_IMAGE = 4
@@ -41,10 +41,11 @@ SYMBOLS = [
 # every symbol include/gsplat_train.h declares
 TRAIN_SYMBOLS = ["gs_ssim_window", "gs_loss_workspace_bytes", "gs_main_loss", "gs_adam_step",
                  "gs_adam_schedule_row", "gs_adam_step_scheduled", "gs_adam_advance", "gs_stage_f32",
-                 "gs_copy_indirect_f32", "gs_sched_lr"]
+                 "gs_copy_indirect_f32", "gs_sched_lr", "gs_tile_balance_workspace_bytes", "gs_tile_balance"]
 # every symbol include/gsplat_densify.h declares
 DENSIFY_SYMBOLS = ["gs_densify_stats", "gs_densify_workspace_bytes", "gs_densify_plan",
-                   "gs_densify_apply", "gs_reset_opacity"]
+                   "gs_densify_apply", "gs_reset_opacity", "gs_sample_workspace_bytes", "gs_sample",
+                   "gs_relocate_workspace_bytes", "gs_relocate"]
 
 
 class GsCamera(C.Structure):
@@ -84,6 +85,14 @@ def lib() -> C.CDLL:
         l.gs_loss_workspace_bytes.argtypes = [C.c_int, C.c_int]
         l.gs_densify_workspace_bytes.restype = C.c_size_t
         l.gs_densify_workspace_bytes.argtypes = [C.c_int]
+        for fn, args in (("gs_tile_balance", [C.c_int] * 2), ("gs_sample", [C.c_int] * 2),
+                         ("gs_relocate", [C.c_int] * 2)):
+            getattr(l, fn + "_workspace_bytes").restype = C.c_size_t
+            getattr(l, fn + "_workspace_bytes").argtypes = args
+        vp = C.c_void_p
+        l.gs_tile_balance.argtypes = [C.c_int] * 3 + [vp, vp, C.c_float, vp, vp, vp, C.c_uint32, vp, C.c_size_t, vp]
+        l.gs_sample.argtypes = [C.c_int, C.c_int, vp, C.c_int64, vp, C.c_int, vp, vp, vp, C.c_size_t, vp]
+        l.gs_relocate.argtypes = [C.c_int] * 3 + [vp, vp, C.c_float, vp, vp, vp, vp, C.c_size_t, vp]
         l.gs_sched_lr.restype = C.c_float
         l.gs_sched_lr.argtypes = [C.c_float, C.c_float, C.c_int, C.c_int]
         _lib = l
@@ -665,6 +674,35 @@ def copy_indirect_f32(dst_dev, src_ptr_pinned, count):
                                       _stream()), "gs_copy_indirect_f32")
 
 
+def tile_balance(W, H, packed, tile_bins, scale=1.0, flags=0, want_grad=True, out=None, workspace=None):
+    """Balance loss of a frame's tile lists (gs_tile_balance): scale * T sum_t (n_t / M) (S_t / S), n_t entries and S_t
+    opacity of tile t's list.  packed [N, 12] and tile_bins [T, 2]: the frame's binning (Binned.packed, .tile_bins).
+    flags: GS_FLAG_LOGIT_OPACITY (gradient w.r.t. the logits), GS_FLAG_ACCUMULATE_GRADS (needs out).
+    -> (loss [1], counts [T] int32, v_opacity [N] or None)."""
+    dev = packed.device
+    N, tiles = packed.shape[0], ((W + GS_TILE - 1) // GS_TILE) * ((H + GS_TILE - 1) // GS_TILE)
+    if packed.dtype != torch.float32 or packed.shape != (N, GS_SPLAT_DWORDS):
+        raise ValueError("packed must be float32 [N, %d]" % GS_SPLAT_DWORDS)
+    if tile_bins.dtype != torch.int32 or tile_bins.shape != (tiles, 2) or tile_bins.device != dev:
+        raise ValueError("tile_bins must be int32 [%d, 2] on %s" % (tiles, dev))
+    if out is None:
+        if flags & GS_FLAG_ACCUMULATE_GRADS:
+            raise ValueError("GS_FLAG_ACCUMULATE_GRADS adds to a v_opacity of the caller's: pass out")
+        out = (torch.empty(1, device=dev, dtype=torch.float32), torch.empty(tiles, device=dev, dtype=torch.int32),
+               torch.empty(N, device=dev, dtype=torch.float32) if want_grad else None)
+    loss, counts, v = out
+    for t, n, dt in ((loss, 1, torch.float32), (counts, tiles, torch.int32), (v, N, torch.float32)):
+        if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev):
+            raise ValueError("out must be (float32 [1], int32 [%d], float32 [%d]) on %s" % (tiles, N, dev))
+    with torch.cuda.device(dev):
+        need = lib().gs_tile_balance_workspace_bytes(W, H)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+        _check(lib().gs_tile_balance(W, H, N, _p(packed), _p(tile_bins), scale, _p(loss), _p(counts), _p(v), flags,
+                                     _p(workspace), workspace.numel(), _stream()), "gs_tile_balance")
+    return loss, counts, v
+
+
 def sched_lr(lr_init, lr_final, max_steps, step):
     return float(lib().gs_sched_lr(lr_init, lr_final, max_steps, step))
 
@@ -762,6 +800,95 @@ def reset_opacity(opacity_logits, reset_value=0.2, exp_avg=None, exp_avg_sq=None
     _check(lib().gs_reset_opacity(C.c_int(opacity_logits.numel()), C.c_float(reset_value),
                                   _p(opacity_logits), _p(exp_avg), _p(exp_avg_sq), _stream()),
            "gs_reset_opacity")
+
+
+class GsSampleConfig(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("flags", C.c_uint32), ("temperature", C.c_float), ("top_k", C.c_int32),
+                ("top_p", C.c_float), ("min_p", C.c_float), ("temperature_rows", C.c_void_p),
+                ("top_k_rows", C.c_void_p), ("top_p_rows", C.c_void_p), ("min_p_rows", C.c_void_p)]
+
+
+_SAMPLE_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, opacity=False, out=None,
+           workspace=None):
+    """Indices drawn from given random numbers (gs_sample).  logits [R, V] (or [V]) float32 / float16 / bfloat16, rows
+    of any stride; uniforms [R, D] (or [D]) float32 in [0, 1).  temperature, top_k, top_p, min_p: a number for all
+    rows, or a GPU tensor [R] (float32, top_k int32).  opacity: the logits are opacity logits, the weights sigmoids.
+    -> ids int32 like uniforms; -1 where a row has no candidate."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the GPU")
+    dev, shape = logits.device, uniforms.shape
+    if logits.dim() == 1:
+        logits = logits[None]
+    if uniforms.dim() == 1:
+        uniforms = uniforms[None]
+    if logits.dim() != 2 or uniforms.dim() != 2 or uniforms.shape[0] != logits.shape[0]:
+        raise ValueError("logits [R, V] and uniforms [R, D] (or [V] and [D]) needed, got %s and %s"
+                         % (tuple(logits.shape), tuple(shape)))
+    R, V = logits.shape
+    if logits.dtype not in _SAMPLE_DTYPES:
+        raise ValueError("logits must be float32, float16 or bfloat16, not %s" % logits.dtype)
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("the entries of a row must be adjacent (stride 1)")
+    if R > 1 and logits.stride(0) < V:
+        raise ValueError("rows of the logits must not overlap")
+    if uniforms.dtype != torch.float32 or uniforms.device != dev or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be contiguous float32 on %s" % dev)
+    cfg = GsSampleConfig(_SAMPLE_DTYPES[logits.dtype], GS_FLAG_LOGIT_OPACITY if opacity else 0, 1.0, 0, 1.0, 0.0)
+    for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if isinstance(v, torch.Tensor):
+            if v.shape != (R,) or v.device != dev or not v.is_contiguous() or \
+                    v.dtype != (torch.int32 if name == "top_k" else torch.float32):
+                raise ValueError("%s must be a number or a contiguous %s tensor [%d] on %s"
+                                 % (name, "int32" if name == "top_k" else "float32", R, dev))
+            setattr(cfg, name + "_rows", v.data_ptr())
+        elif v is not None:
+            setattr(cfg, name, v)
+    if out is None:
+        out = torch.empty(shape, device=dev, dtype=torch.int32)
+    elif out.shape != shape or out.dtype != torch.int32 or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous int32 %s on %s" % (tuple(shape), dev))
+    with torch.cuda.device(dev):
+        need = lib().gs_sample_workspace_bytes(R, V)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
+        _check(lib().gs_sample(R, V, logits.data_ptr(), logits.stride(0) if R > 1 else V, C.byref(cfg),
+                               uniforms.shape[1], _p(uniforms), _p(out), _p(workspace), workspace.numel(), _stream()),
+               "gs_sample")
+    return out
+
+
+def relocate(params, exp_avg, exp_avg_sq, targets, sources, min_opacity=0.005, workspace=None):
+    """Rows `targets` become copies of rows `sources` (int32 [n] each), in place: a source and its copies together keep
+    the source's opacity and extent, the moments of the rows written become 0 (gs_relocate).  params / exp_avg /
+    exp_avg_sq: lists of the six tensors [means, log_scales, quats, opacity_logits, features_dc, features_rest] (the
+    moment lists may be None).  Pairs with an index outside [0, N) change nothing, as do pairs whose source is a target
+    and all but the first pair of a target."""
+    means, dev = params[0], params[0].device
+    N, n = means.shape[0], targets.numel()
+    rest = params[5] if len(params) > 5 else None
+    K = 1 + (rest.shape[1] if rest is not None and rest.numel() > 0 else 0)
+    for t in (targets, sources):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != dev or not t.is_contiguous():
+            raise ValueError("targets and sources must be contiguous int32 [n] on %s" % dev)
+    lens = (3, 3, 4, 1, 3, 3 * (K - 1))
+    for tensors in (params, exp_avg, exp_avg_sq):
+        for t, k in zip(tensors or (), lens):
+            if t is not None and (t.numel() != N * k or t.device != dev):
+                raise ValueError("a Gaussian set of %d rows and K = %d needs tensors of %s floats a row on %s"
+                                 % (N, K, lens, dev))
+    if N == 0 or n == 0:
+        return
+    with torch.cuda.device(dev):
+        need = lib().gs_relocate_workspace_bytes(N, n)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+        sets = [_set(t) if t else None for t in (params, exp_avg, exp_avg_sq)]
+        _check(lib().gs_relocate(N, K, n, _p(targets), _p(sources), min_opacity,
+                                 *[C.byref(s) if s is not None else None for s in sets], _p(workspace),
+                                 workspace.numel(), _stream()), "gs_relocate")
 
 
 # ---------------------------------------------------------------------------------------------
