@@ -214,6 +214,31 @@ void resetOpacity(torch::Tensor &opacities, float resetValue,
                   c10::optional<torch::Tensor> expAvg = c10::nullopt,
                   c10::optional<torch::Tensor> expAvgSq = c10::nullopt);
 
+// A fixed budget of Gaussians (include/gsplat_densify.h: gs_sample, gs_relocate; gsplat_train.h: gs_tile_balance) — the
+// strategy beside the reference's densification by thresholds.
+//   sampleIndices      int32 [R, D] drawn from the rows of logits [R, V] (float32 / float16 / bfloat16) with the given
+//                      uniforms [R, D]; settings per row as [R] tensors, absent ones off; opacity: weights are sigmoids
+//   relocateGaussians  rows `targets` become copies of rows `sources` (int32 [n]), in place; a source and its copies
+//                      together keep its opacity and extent; moments (may be empty) of the rows written become 0
+//   TileBalance        T sum_t (n_t / M) (S_t / S) of a frame's tile lists as an autograd node of the opacities (or
+//                      their logits) the records were packed from; returns a 0-dim tensor
+torch::Tensor sampleIndices(const torch::Tensor &logits, const torch::Tensor &uniforms,
+                            const c10::optional<torch::Tensor> &temperature = c10::nullopt,
+                            const c10::optional<torch::Tensor> &topK = c10::nullopt,
+                            const c10::optional<torch::Tensor> &topP = c10::nullopt,
+                            const c10::optional<torch::Tensor> &minP = c10::nullopt, bool opacity = false);
+void relocateGaussians(const std::vector<torch::Tensor> &params, const std::vector<torch::Tensor> &expAvg,
+                       const std::vector<torch::Tensor> &expAvgSq, const torch::Tensor &targets,
+                       const torch::Tensor &sources, float minOpacity);
+class TileBalance : public torch::autograd::Function<TileBalance> {
+public:
+    static torch::Tensor forward(torch::autograd::AutogradContext *ctx, torch::Tensor opacities, torch::Tensor packed,
+                                 torch::Tensor tileBins, int64_t imgHeight, int64_t imgWidth, bool opacityIsLogit);
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::tensor_list grad_outputs);
+};
+torch::Tensor tileBalance(const torch::Tensor &opacities, const BinnedLists &lists, bool opacityIsLogit = false);
+
 // SURVEY.md §8e — the one exchange step of the camera-per-rank path for a C++ caller: a sum
 // all-reduce of the flat gradient buffer (RCCL over xGMI, include/gsplat_dist.h) enqueued on the
 // current torch HIP stream, i.e. right behind the backward kernels that filled the buffer.

@@ -937,8 +937,121 @@ void resetOpacity(Tensor &opacities, float resetValue, c10::optional<Tensor> exp
                  "gs_reset_opacity");
 }
 
+// ---- a fixed budget of Gaussians: draw sources, relocate onto them; the tile lists' balance loss -----------------
+Tensor sampleIndices(const Tensor &logits, const Tensor &uniforms, const c10::optional<Tensor> &temperature,
+                     const c10::optional<Tensor> &topK, const c10::optional<Tensor> &topP,
+                     const c10::optional<Tensor> &minP, bool opacity) {
+    GS_CHECK_DEV(logits); GS_CHECK_DEV(uniforms); GS_CHECK_F32(uniforms);
+    TORCH_CHECK(logits.dim() == 2 && uniforms.dim() == 2 && logits.size(0) == uniforms.size(0),
+                "logits [R, V] and uniforms [R, D] expected");
+    TORCH_CHECK(uniforms.is_contiguous() && uniforms.device() == logits.device(),
+                "uniforms must be contiguous and on the logits' device");
+    const int64_t R = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(R <= INT32_MAX && V <= INT32_MAX && uniforms.size(1) <= INT32_MAX, "at most 2^31 - 1 rows, entries, draws");
+    TORCH_CHECK(V <= 1 || logits.stride(1) == 1, "the entries of a row must be adjacent");
+    TORCH_CHECK(R <= 1 || logits.stride(0) >= V, "rows of the logits must not overlap");
+    GsSampleConfig c = {GS_DTYPE_F32, opacity ? GS_FLAG_LOGIT_OPACITY : 0u, 1.0f, 0, 1.0f, 0.0f,
+                        nullptr, nullptr, nullptr, nullptr};
+    switch (logits.scalar_type()) {
+    case torch::kFloat32: break;
+    case torch::kFloat16: c.dtype = GS_DTYPE_F16; break;
+    case torch::kBFloat16: c.dtype = GS_DTYPE_BF16; break;
+    default: TORCH_CHECK(false, "logits must be float32, float16 or bfloat16");
+    }
+    auto rows = [&](const c10::optional<Tensor> &t, torch::ScalarType type) -> const void * {
+        if (!t) return nullptr;
+        TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->dim() == 1 && t->size(0) == R &&
+                        t->is_contiguous(), "per-row settings must be contiguous [R] (top_k int32, the others float32)");
+        return t->data_ptr();
+    };
+    c.temperature_rows = (const float *)rows(temperature, torch::kFloat32);
+    c.top_k_rows = (const int32_t *)rows(topK, torch::kInt32);
+    c.top_p_rows = (const float *)rows(topP, torch::kFloat32);
+    c.min_p_rows = (const float *)rows(minP, torch::kFloat32);
+    c10::DeviceGuard guard(logits.device());
+    Tensor ids = torch::empty(uniforms.sizes(), uniforms.options().dtype(torch::kInt32));
+    const size_t bytes = gs_sample_workspace_bytes((int)R, (int)V);
+    Tensor ws = torch::empty({(int64_t)bytes}, uniforms.options().dtype(torch::kUInt8));
+    check_status(gs_sample((int)R, (int)V, logits.data_ptr(), R > 1 ? logits.stride(0) : V, &c, (int)uniforms.size(1),
+                           fptr(uniforms), ids.data_ptr<int32_t>(), ws.data_ptr(), bytes, current_stream()), "gs_sample");
+    return ids;
+}
+
+Tensor TileBalance::forward(AutogradContext *ctx, Tensor opacities, Tensor packed, Tensor tileBins, int64_t imgHeight,
+                            int64_t imgWidth, bool opacityIsLogit) {
+    GS_CHECK_DEV(opacities); GS_CHECK_DEV(packed); GS_CHECK_DEV(tileBins);
+    GS_CHECK_F32(opacities); GS_CHECK_F32(packed); GS_CHECK_I32(tileBins);
+    const int64_t N = packed.size(0), tiles = ((imgWidth + 15) / 16) * ((imgHeight + 15) / 16);
+    TORCH_CHECK(packed.dim() == 2 && packed.size(1) == GS_SPLAT_DWORDS && packed.is_contiguous(), "packed must be [N, 12]");
+    TORCH_CHECK(tileBins.numel() == 2 * tiles && tileBins.is_contiguous(), "tileBins must be [tiles, 2]");
+    TORCH_CHECK(opacities.numel() == N, "one opacity per record");
+    TORCH_CHECK(packed.device() == opacities.device() && tileBins.device() == opacities.device(), "one device expected");
+    c10::DeviceGuard guard(packed.device());
+    const bool want = opacities.requires_grad();
+    Tensor loss = torch::empty({}, packed.options());
+    Tensor v = want ? torch::empty(opacities.sizes(), packed.options()) : Tensor();
+    const size_t bytes = gs_tile_balance_workspace_bytes((int)imgWidth, (int)imgHeight);
+    Tensor ws = torch::empty({(int64_t)bytes}, packed.options().dtype(torch::kUInt8));
+    check_status(gs_tile_balance((int)imgWidth, (int)imgHeight, (int)N, fptr(packed), tileBins.data_ptr<int32_t>(), 1.0f,
+                                 fptr_mut(loss), nullptr, want ? fptr_mut(v) : nullptr,
+                                 opacityIsLogit ? GS_FLAG_LOGIT_OPACITY : 0u, ws.data_ptr(), bytes, current_stream()),
+                 "gs_tile_balance");
+    if (want) ctx->save_for_backward({v});
+    return loss;
+}
+
+tensor_list TileBalance::backward(AutogradContext *ctx, tensor_list grad_outputs) {
+    const auto saved = ctx->get_saved_variables();
+    return {saved.empty() ? Tensor() : saved[0] * grad_outputs[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+}
+
+Tensor tileBalance(const Tensor &opacities, const BinnedLists &lists, bool opacityIsLogit) {
+    return TileBalance::apply(opacities, lists.packed, lists.tileBins, (int64_t)lists.height, (int64_t)lists.width,
+                              opacityIsLogit);
+}
+
+void relocateGaussians(const std::vector<Tensor> &params, const std::vector<Tensor> &expAvg,
+                       const std::vector<Tensor> &expAvgSq, const Tensor &targets, const Tensor &sources,
+                       float minOpacity) {
+    TORCH_CHECK(params.size() == 6, "six parameter tensors expected");
+    TORCH_CHECK(expAvg.empty() || expAvg.size() == 6, "six exp_avg tensors (or none) expected");
+    TORCH_CHECK(expAvgSq.empty() || expAvgSq.size() == 6, "six exp_avg_sq tensors (or none) expected");
+    const int64_t N = params[0].size(0), K = 1 + (params[5].numel() > 0 ? params[5].size(1) : 0);
+    const int64_t lens[6] = {3, 3, 4, 1, 3, 3 * (K - 1)};
+    for (const auto *set : {&params, &expAvg, &expAvgSq})
+        for (size_t i = 0; i < set->size(); i++) {
+            const Tensor &t = (*set)[i];
+            TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() &&
+                            t.device() == params[0].device() && t.numel() == N * lens[i],
+                        "contiguous float32 GPU tensors of N rows expected");
+        }
+    for (const Tensor *t : {&targets, &sources})
+        TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kInt32 && t->is_contiguous() && t->dim() == 1 &&
+                        t->numel() == targets.numel() && t->device() == params[0].device(),
+                    "targets and sources must be contiguous int32 [n]");
+    const int64_t n = targets.numel();
+    TORCH_CHECK(N <= INT32_MAX && n <= INT32_MAX, "at most 2^31 - 1 rows and pairs");
+    if (N == 0 || n == 0) return;
+    c10::DeviceGuard guard(params[0].device());
+    const size_t bytes = gs_relocate_workspace_bytes((int)N, (int)n);
+    Tensor ws = torch::empty({(int64_t)bytes}, params[0].options().dtype(torch::kUInt8).requires_grad(false));
+    const GsGaussianSet p = as_set(params), m = as_set(expAvg), v = as_set(expAvgSq);
+    check_status(gs_relocate((int)N, (int)K, (int)n, targets.data_ptr<int32_t>(), sources.data_ptr<int32_t>(), minOpacity,
+                             &p, &m, &v, ws.data_ptr(), bytes, current_stream()), "gs_relocate");
+}
+
 // ---- Python-visible registration (torch.ops.opensplat_amd.*) -------------------------------------
 namespace {
+
+Tensor op_tile_balance(const Tensor &opacities, const Tensor &packed, const Tensor &tileBins, int64_t imgHeight,
+                       int64_t imgWidth, bool opacityIsLogit) {
+    return TileBalance::apply(opacities, packed, tileBins, imgHeight, imgWidth, opacityIsLogit);
+}
+
+void op_relocate(std::vector<Tensor> params, std::vector<Tensor> expAvg, std::vector<Tensor> expAvgSq,
+                 const Tensor &targets, const Tensor &sources, double minOpacity) {
+    relocateGaussians(params, expAvg, expAvgSq, targets, sources, (float)minOpacity);
+}
 
 std::vector<Tensor> op_project_gaussians(const Tensor &means, const Tensor &scales, double globScale,
                                          const Tensor &quats, const Tensor &viewMat,
@@ -1380,4 +1493,13 @@ TORCH_LIBRARY(opensplat_amd, m) {
     m.def("adam_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, "
           "float[] lrs, int step) -> ()",
           &op_adam_step);
+    m.def("sample_indices(Tensor logits, Tensor uniforms, Tensor? temperature=None, Tensor? top_k=None, "
+          "Tensor? top_p=None, Tensor? min_p=None, bool opacity=False) -> Tensor",
+          &sampleIndices);
+    m.def("tile_balance(Tensor opacities, Tensor packed, Tensor tile_bins, int img_height, int img_width, "
+          "bool opacity_is_logit=False) -> Tensor",
+          &op_tile_balance);
+    m.def("relocate(Tensor(a!)[] params, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor targets, "
+          "Tensor sources, float min_opacity) -> ()",
+          &op_relocate);
 }

@@ -137,6 +137,24 @@ def adam_step(params, grads, exp_avg, exp_avg_sq, lrs, step):
                    [float(x) for x in lrs], int(step))
 
 
+def sample_indices(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, opacity=False):
+    """int32 [R, D] indices of the rows of logits [R, V], drawn with the given uniforms [R, D]; settings per row as
+    [R] GPU tensors (gs_sample; opacity: the weights are the sigmoids of the logits)."""
+    return _ops.sample_indices(logits, uniforms, temperature, top_k, top_p, min_p, bool(opacity))
+
+
+def tile_balance(opacities, packed, tile_bins, img_height, img_width, opacity_is_logit=False):
+    """Balance loss of a frame's tile lists (gs_tile_balance) as an autograd node of the opacities (or logits) the
+    records `packed` were built from; returns a 0-dim tensor."""
+    return _ops.tile_balance(opacities, packed, tile_bins, int(img_height), int(img_width), bool(opacity_is_logit))
+
+
+def relocate(params, exp_avg, exp_avg_sq, targets, sources, min_opacity=0.005):
+    """Rows `targets` become copies of rows `sources`, in place (gs_relocate); lists as in densify(), all six tensors
+    (featuresRest empty for K = 1)."""
+    _ops.relocate(list(params), list(exp_avg or []), list(exp_avg_sq or []), targets, sources, float(min_opacity))
+
+
 def densify_stats(xys_grad, radii, last_height, last_width, stats=None):
     """Model::afterTrain's per-iteration statistics (model.cpp:317-337).  stats = (xysGradNorm,
     visCounts, max2DSize) from the previous call, or None right after a refinement; returns them."""

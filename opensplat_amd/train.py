@@ -66,6 +66,7 @@ class Trainer:
     LR = dict(means=0.00016, scales=0.005, quats=0.001, features_dc=0.0025,
               features_rest=0.000125, opacities=0.05)
     MEANS_LR_FINAL = 0.0000016
+    COPY_SPREAD = 0.2   # strategy="relocate": how far a copy leaves its source, in standard deviations
 
     def __init__(self, means, log_scales, quats, opacity_logits, features_dc, features_rest,
                  device, max_steps: int = 30000, ssim_weight: float = 0.2, refine_every: int = 100,
@@ -75,7 +76,9 @@ class Trainer:
                  num_cameras: int = 1, morton_order: bool = False, num_downscales: int = 2,
                  resolution_schedule: int = 3000, sh_degree_interval: int = 1000,
                  reference_alpha_reset: bool = False, grad_buckets: int = 4, exchange: str = "auto",
-                 deterministic: bool = False, segmented: bool = True, experimental_graph: bool = False):
+                 deterministic: bool = False, segmented: bool = True, experimental_graph: bool = False,
+                 strategy: str = "thresholds", max_gaussians: int = 0, min_opacity: float = 0.005,
+                 source_temperature: float = 1.0, source_top_p: float = 1.0, balance_weight: float = 0.0):
         """Parameters as Model holds them (model.hpp): means [N,3], log-scales [N,3], raw quats
         [N,4], opacity logits [N] or [N,1], featuresDc [N,3], featuresRest [N,K-1,3].
         segmented: on frames of few tiles the compositing backward runs the pieces of a tile's list side by
@@ -86,6 +89,23 @@ class Trainer:
         explained (profiles/HISTORY.md).  The building blocks it is made of — gs_adam_step_scheduled,
         gs_stage_f32, gs_copy_indirect_f32 — are supported and tested eagerly (tests/test_gpu_train_blocks.py)."""
         graph = experimental_graph
+        # How the set is refined.  "thresholds": the reference's split / duplicate / cull (model.cpp:311-494).
+        # "relocate": a budget — every refine_every steps the Gaussians whose opacity has fallen to min_opacity become
+        # copies of sources drawn in proportion to their opacity (gs_sample, sharpened by source_temperature and cut to
+        # the strongest that hold source_top_p of the opacity), and the set grows by a twentieth of such copies until
+        # it holds max_gaussians (0: it does not grow).  Source and copies keep the source's opacity and extent
+        # (gs_relocate).  No statistics, no alpha reset.
+        if strategy not in ("thresholds", "relocate"):
+            raise ValueError("strategy must be 'thresholds' or 'relocate', not %r" % (strategy,))
+        if not 0.0 < min_opacity < 1.0 or not source_temperature > 0.0 or not 0.0 < source_top_p <= 1.0:
+            raise ValueError("min_opacity in (0, 1), source_temperature > 0, source_top_p in (0, 1] needed")
+        if strategy == "relocate" and reference_alpha_reset:
+            raise ValueError("strategy='relocate' has no alpha reset")
+        self.strategy, self.max_gaussians, self.min_opacity = strategy, int(max_gaussians), float(min_opacity)
+        self.source_temperature, self.source_top_p = float(source_temperature), float(source_top_p)
+        # weight of the tile lists' balance loss (gs_tile_balance) in the step's loss, mean over the cameras like the
+        # image loss; its gradient joins the opacities' behind every backward
+        self.balance_weight = float(balance_weight)
         self.segmented, self._ckpt = segmented, cabi.Checkpoints()
         t = lambda a: torch.as_tensor(np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a,
                                       dtype=torch.float32).to(device)
@@ -211,6 +231,8 @@ class Trainer:
         self.loss_ws = torch.empty(cabi.lib().gs_loss_workspace_bytes(W, H), device=dev,
                                    dtype=torch.uint8)
         self.loss_out = (torch.empty(3, **f), torch.empty((H, W, 3), **f))
+        if self.balance_weight:
+            self.balance_out, self.balance_ws = self._balance_buffers(W, H)
         self._shape = (W, H)
         self._buf_gen += 1
         self._graphs.clear()
@@ -228,6 +250,18 @@ class Trainer:
             self._g_done = torch.cuda.Event()
             if self._g_stream is None:
                 self._g_stream = torch.cuda.Stream()
+
+    def _balance_buffers(self, W, H):
+        """-> (loss [1], entries per tile, the opacities' gradient) and a workspace, for _balance."""
+        dev = self.dev
+        tiles = ((W + cabi.GS_TILE - 1) // cabi.GS_TILE) * ((H + cabi.GS_TILE - 1) // cabi.GS_TILE)
+        return (torch.empty(1, device=dev), torch.empty(tiles, device=dev, dtype=torch.int32), self.grads.v_opacity), \
+            torch.empty(cabi.lib().gs_tile_balance_workspace_bytes(W, H), device=dev, dtype=torch.uint8)
+
+    def _balance(self, W, H, b, scale, out, workspace):
+        """The balance loss of the frame's lists, its gradient added to the opacities' (behind gaussian_backward)."""
+        cabi.tile_balance(W, H, b.packed, b.tile_bins, scale * self.balance_weight,
+                          cabi.GS_FLAG_LOGIT_OPACITY | cabi.GS_FLAG_ACCUMULATE_GRADS, out=out, workspace=workspace)
 
     def render(self, cam: dict, background, degrees_to_use: int):
         """Model::forward (model.cpp:83-225) for one camera -> clamped rgb [H, W, 3]."""
@@ -288,6 +322,8 @@ class Trainer:
                                    cam_pos, self.K, deg, p["radii"], rgb_raw, self.bwd_ws,
                                    dict(self.gout, v_dc=fx.v_color(0), v_rest=None),
                                    flags | cabi.GS_FLAG_EMIT_VCOLOR, v_xy=self.v_xy)
+            if self.balance_weight:
+                self._balance(W, H, b, 1.0 / self.world, self.balance_out, self.balance_ws)
             fx.start(self.grads)
             sh = self.grads.sh_numel
             # (lo, hi, wait-and-prepare): the SH block first — its Adam step overlaps the geometry all-reduce
@@ -297,6 +333,8 @@ class Trainer:
         cabi.gaussian_backward(gcam, self.means, self.log_scales, self.quats, self.opacity_logits,
                                cam_pos, self.K, deg, p["radii"], rgb_raw, self.bwd_ws, self.gout, flags,
                                v_xy=self.v_xy)
+        if self.balance_weight:
+            self._balance(W, H, b, 1.0 / self.world, self.balance_out, self.balance_ws)
         # start the exchange; optimizer_step() consumes it bucket by bucket
         self._pending = [(lo, hi, (lambda w=w: dist.wait_all(w)))
                          for lo, hi, w in dist.allreduce_buckets_async(self.grads, self.grad_buckets)] \
@@ -421,6 +459,8 @@ class Trainer:
         cabi.gaussian_backward(gcam, self.means, self.log_scales, self.quats, self.opacity_logits, pos,
                                self.K, deg, p["radii"], p["rgb_raw"], self.bwd_ws, self.gout, flags,
                                v_xy=self.v_xy, viewmat_dev=vm, projmat_dev=pm)
+        if self.balance_weight:
+            self._balance(W, H, b, 1.0, self.balance_out, self.balance_ws)
         off = cabi.lib().gs_bin_num_isects_offset(W, H)
         guard = self.bin_ws.bufs["ws"][off:off + 4].view(torch.int32)
         groups = [g[:5] for g in self.adam_groups()]
@@ -517,6 +557,9 @@ class Trainer:
 
         if getattr(self, "_lane_key", None) != (W, H, self.N):
             self._lanes = [CameraLane(self.N, W, H, self.dev, clamped=True, loss=True) for _ in range(2)]
+            if self.balance_weight:
+                for L in self._lanes:
+                    L.balance = self._balance_buffers(W, H)
             self._lane_key = (W, H, self.N)
         return self._lanes
 
@@ -571,7 +614,7 @@ class Trainer:
                 if hit is None or hit[0] != key:
                     hit = cam["_cam_pos_dev"] = (key, torch.from_numpy(cam_pos).to(self.dev))
                 pos_dev.append(hit[1])
-        collect = step is not None and step < self.stop_split_at
+        collect = step is not None and step < self.stop_split_at and self.strategy == "thresholds"
         first_stats = [collect and self._stats is None]
         if first_stats[0]:
             self._stats = tuple(torch.zeros(N, device=self.dev, dtype=torch.float32) for _ in range(3))
@@ -605,6 +648,8 @@ class Trainer:
                 cabi.gaussian_backward(gcam, self.means, self.log_scales, self.quats, self.opacity_logits, cam_pos,
                                        self.K, degrees_to_use, L.g["radii"], L.g["rgb_raw"], L.bwd_ws, gout, gflags,
                                        v_xy=L.v_xy)
+                if self.balance_weight:
+                    self._balance(W, H, L.b, scale, *L.balance)
                 if fx is not None:
                     fx.start_camera(j)
                 if collect:
@@ -650,6 +695,10 @@ class Trainer:
         step refined the Gaussian set, else None."""
         gcam, cam_pos, p, rgb_raw, b, f, flags, deg, background, W, H = self._ctx
         N, dev = self.N, self.dev
+        if self.strategy == "relocate":
+            if step % self.refine_every == 0 and self.warmup_length < step < self.stop_split_at:
+                return self._relocate(step)
+            return None
         if not self._visible and self.world == 1:   # model.cpp:315 (with a batch, another rank's
             return None                             # camera may see Gaussians: the step counts)
         if getattr(self, "_batch_stats_step", None) == step:
@@ -684,6 +733,58 @@ class Trainer:
                                        self.exp_avg_sq.v_opacity)
             self._stats = None           # model.cpp:482-484
         return counts
+
+    def _draw_sources(self, dead, n, gen):
+        """n indices among the Gaussians that are not dead, in proportion to their opacity (-1: there are none)."""
+        weights = torch.where(dead, -torch.inf, self.opacity_logits)
+        return cabi.sample(weights, torch.rand(n, device=self.dev, generator=gen), self.source_temperature,
+                           top_p=self.source_top_p, opacity=True)
+
+    def _copy_sources(self, targets, sources, gen):
+        """gs_relocate on parameters and moments, then the copies leave their sources by a part of their extent: equal
+        Gaussians with equal gradients would stay together for good."""
+        cabi.relocate(*[self._param_list(b) for b in (self.params, self.exp_avg, self.exp_avg_sq)], targets, sources,
+                      self.min_opacity)
+        t = targets.long()
+        q = torch.nn.functional.normalize(self.quats[t], dim=1)
+        v = torch.randn((t.numel(), 3), device=self.dev, generator=gen) * self.log_scales[t].exp()
+        u, w = q[:, 1:], q[:, :1]
+        c = 2.0 * torch.linalg.cross(u, v)
+        moved = self.means[t] + self.COPY_SPREAD * (v + w * c + torch.linalg.cross(u, c))
+        self.means[t] = torch.where((sources >= 0)[:, None], moved, self.means[t])
+
+    def _relocate(self, step):
+        """strategy="relocate": -> dict(relocated, added).  The draws come from the step number and the parameters alone:
+        ranks with equal parameters take equal decisions.  One host synchronisation, to read how many are dead."""
+        gen = torch.Generator(device=self.dev).manual_seed(1_000_003 * step)
+        logit = float(np.log(self.min_opacity / (1.0 - self.min_opacity)))
+        dead = self.opacity_logits <= logit
+        targets = dead.nonzero().view(-1).int()
+        alive = self.N - targets.numel()
+        if alive == 0:
+            return dict(relocated=0, added=0)
+        if targets.numel():
+            self._copy_sources(targets, self._draw_sources(dead, targets.numel(), gen), gen)
+        grow = min(self.max_gaussians, self.N + (self.N + 19) // 20) - self.N
+        if grow > 0:
+            # (drawn from the whole new set: a share that the copying left at the bound still counts)
+            old_n = self.N
+            sources = self._draw_sources(self.opacity_logits < logit, grow, gen)
+            for name in ("params", "exp_avg", "exp_avg_sq"):
+                new, old = dist.GradBuffer(old_n + grow, self.K, self.dev), getattr(self, name)
+                for a, t in zip(self._param_list(new), self._param_list(old)):
+                    if t is not None:
+                        a[:old_n].copy_(t)
+                        a[old_n:].zero_()
+                setattr(self, name, new)
+            self.N = old_n + grow
+            # (a row that found no source stays invisible until a later relocation)
+            self.params.v_opacity[old_n:] = logit
+            self._copy_sources(torch.arange(old_n, self.N, device=self.dev, dtype=torch.int32), sources, gen)
+            self.grads = dist.GradBuffer(self.N, self.K, self.dev)
+            self._shape = None               # per-N render buffers are rebuilt on the next render
+            self._graphs.clear()             # (captured graphs point at the replaced buffers)
+        return dict(relocated=targets.numel(), added=max(grow, 0))
 
     def _refine(self, step, W, H):
         gn, vc, m2 = self._stats

@@ -69,6 +69,10 @@ def main():
                     help="the reference's CLI defaults as they are (--sh-degree-interval 1000, "
                          "--resolution-schedule 3000: what `opensplat -n 7000` runs) instead of schedules "
                          "scaled to the run's length")
+    ap.add_argument("--strategy", choices=("thresholds", "relocate"), default="thresholds",
+                    help="how Trainer refines the set: the reference's densification, or relocation at a budget")
+    ap.add_argument("--max-gaussians", type=int, default=0, help="--strategy relocate: the budget the set grows to")
+    ap.add_argument("--balance-weight", type=float, default=0.0, help="weight of the tile lists' balance loss")
     ap.add_argument("--cpu-baseline", action="store_true",
                     help="also time the reference's own CPU chain (oracle/_ref) on one iteration of the initial "
                          "set at every resolution of the schedule, and extrapolate the run")
@@ -113,7 +117,8 @@ def main():
         dict(sh_degree_interval=max(a.iters // 4, 1), resolution_schedule=max(a.iters // 6, 1))
     T = train.Trainer(*init, DEV, max_steps=a.iters, ssim_weight=0.2, num_cameras=n_train,
                       morton_order=True, num_downscales=a.num_downscales, experimental_graph=a.graph,
-                      segmented=not a.no_segments, **sched)
+                      segmented=not a.no_segments, strategy=a.strategy, max_gaussians=a.max_gaussians,
+                      balance_weight=a.balance_weight, **sched)
     n_initial = T.N
     sh_interval = T.sh_degree_interval
 
@@ -166,7 +171,8 @@ def main():
             last_loss = [float(x) for x in loss.cpu()]   # before a refinement reallocates buffers
         c = T.after_train(step)
         if c is not None:
-            refinements.append({"step": step, "added": c["added"], "culled": c["culled"], "gaussians": T.N})
+            refinements.append({"step": step, "gaussians": T.N,
+                                **{k: c[k] for k in ("added", "culled", "relocated") if k in c}})
         if step % max(a.iters // 6, 1) == 0:
             torch.cuda.synchronize()
             train_time += time.time() - t0
