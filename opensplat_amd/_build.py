@@ -59,7 +59,8 @@ def build_hip(force: bool = False) -> str:
             objects.append(s.replace(".hip", ".o"))
             flags = [f for f in HIPCC_FLAGS if f != "-shared"]
             _run([hipcc] + flags + HIPCC_PLAIN_FLAGS + ["-c", s, "-o", objects[-1]])
-        _run([hipcc] + HIPCC_FLAGS + HIP_SOURCES + objects + ["-o", HIP_LIB])
+        # (objects first: a source file name makes hipcc read everything behind it as source)
+        _run([hipcc] + HIPCC_FLAGS + objects + HIP_SOURCES + ["-o", HIP_LIB])
     return HIP_LIB
 
 

@@ -7,11 +7,21 @@
 //   draw    the lowest index whose running sum of kept weights, in index order, exceeds u times the total
 //
 // The kept entries are a prefix of the order up to min_p, so a row's selection is two numbers: a threshold key and how
-// many of the entries that equal it are kept (the lowest indices).  Keys are the 32 bits of the value mapped so that
-// unsigned order is value order; 0 stands for "no candidate".
+// many of the entries that equal it are kept (the lowest indices).  Keys are the value's bits mapped so that unsigned
+// order is value order (a 16-bit type's key sits in the upper half); 0 stands for "no candidate".  A threshold is found
+// digit by digit (11, 11, 10 bits from the top): a histogram of counts (top-k) or of masses (top-p) over the digit among
+// the entries that agree with the digits found, and the digit in which the running total from above reaches its goal.
+// Nothing is sorted.
 //
-// Weights and their sums are 64-bit: an index is right or wrong, and with 5 million candidates and 250 000 draws a
-// 24-bit weight would move a border across a draw several times in every call.  Every sum has a fixed order.
+// Weights are 64-bit: an index is right or wrong, and with 5 million candidates and 250 000 draws a 24-bit weight would
+// move a border across a draw several times in every call.  Their sums are integers: a weight is rounded once, to a
+// multiple of 2^-50 (rows of up to 4096 entries) to 2^-31 (2^31 entries) of the row's largest, so that sums have no
+// order, running sums never decrease, and a histogram's total, a chunk's and a draw's agree to the last bit.
+//
+// Two forms, by the length of a row:
+//   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row)
+//   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*), the last
+//   workgroup of a row to finish a histogram picking the digit
 #include <math.h>
 
 #include "gs_device.h"
@@ -19,31 +29,21 @@
 
 namespace gs {
 
-constexpr int kSeg = 16;                       // entries one thread sums: the grain of the stored running sums
-constexpr int kSelThreads = 1024;
-constexpr int kSelChunk = kSelThreads * kSeg;  // entries a workgroup sums in one step
-
 enum SampleDtype { kF32 = GS_DTYPE_F32, kF16 = GS_DTYPE_F16, kBF16 = GS_DTYPE_BF16 };
 
 struct SampleArgs {
     const void *logits;
     int64_t stride;
     int rows, cols, draws;
+    double unit;                               // a weight of 1 as an integer: 2^50, or less so that cols * unit <= 2^62
     GsSampleConfig cfg;
 };
 
-// What the draws of a row need of its selection.
-struct SampleRow {
-    double total, inv_t, l_max, min_p;
-    uint32_t max_key, threshold, ties;         // kept: key > threshold, and the first `ties` entries with key == threshold
-    uint32_t pad;
-};
-
-// A row's settings; `ok` false: the row draws nothing.
+// A row's settings.  `greedy`: the first of the order alone (largest value, lowest index).
 struct RowSettings {
-    double temperature, top_p, min_p;
-    int64_t top_k;
-    bool ok;
+    double inv_t, top_p, min_p;
+    int top_k;                                 // 0: all
+    bool ok, greedy;
 };
 
 static __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, int r) {
@@ -51,270 +51,878 @@ static __device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, 
     const float t = c.temperature_rows ? c.temperature_rows[r] : c.temperature;
     const float p = c.top_p_rows ? c.top_p_rows[r] : c.top_p;
     const float m = c.min_p_rows ? c.min_p_rows[r] : c.min_p;
-    int64_t k = c.top_k_rows ? c.top_k_rows[r] : c.top_k;
+    const int k = c.top_k_rows ? c.top_k_rows[r] : c.top_k;
     RowSettings s;
     s.ok = t >= 0.0f && !isnan(p) && !isnan(m);
-    if (k <= 0) k = a.cols;
-    // temperature 0, a min_p that nothing reaches, a top_p that asks for no mass: the first of the order alone
-    if (t == 0.0f || m > 1.0f || p <= 0.0f) k = 1;
-    s.top_k = k;
-    s.temperature = t == 0.0f ? 1.0 : (double)t;
-    s.top_p = (p < 1.0f && p > 0.0f) ? (double)p : 1.0;
-    s.min_p = m > 1.0f ? 0.0 : (double)m;
+    s.greedy = t == 0.0f || m > 1.0f || p <= 0.0f || k == 1;
+    s.top_k = (k > 0 && k < a.cols) ? k : 0;
+    s.inv_t = s.greedy ? 1.0 : 1.0 / (double)t;
+    s.top_p = p < 1.0f ? (double)p : 1.0;
+    s.min_p = s.greedy ? 0.0 : (double)m;
     return s;
 }
 
-static __device__ __forceinline__ uint32_t key_of(float x) {
+// ---- keys -------------------------------------------------------------------------------------------------------
+static __device__ __forceinline__ uint32_t key_f32(uint32_t b) {
+    const float x = __uint_as_float(b);
     if (!(x > -INFINITY)) return 0u;           // NaN, -inf
-    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 and 0 are equal values)
+    b = __float_as_uint(x + 0.0f);             // (-0 and 0 are equal values)
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-static __device__ __forceinline__ float value_of(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+// 16-bit types: `b` the raw bits, `inf` the bits of +inf (all beyond it are NaN)
+template <int DT>
+static __device__ __forceinline__ uint32_t key_16(uint32_t b) {
+    constexpr uint32_t inf = DT == kBF16 ? 0x7F80u : 0x7C00u;
+    if ((b & 0x7FFFu) > inf || b == (inf | 0x8000u)) return 0u;
+    if (b == 0x8000u) b = 0u;
+    return ((b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u)) << 16;
 }
+template <int DT>
+static __device__ __forceinline__ float value_of(uint32_t key) {
+    if constexpr (DT == kF32) return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+    const uint32_t h = key >> 16, b = (h & 0x8000u) ? (h & 0x7FFFu) : (~h & 0xFFFFu);
+    if constexpr (DT == kBF16) return __uint_as_float(b << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+}
+template <int DT>
+constexpr int kBytes = DT == kF32 ? 4 : 2;
+template <int DT>
+constexpr int kVec = 16 / kBytes<DT>;          // entries of one 16-byte load (of any alignment)
 
 template <int DT>
-static __device__ __forceinline__ float load_value(const void *row, int64_t i) {
-    if constexpr (DT == kF32) return static_cast<const float *>(row)[i];
-    if constexpr (DT == kBF16) return __uint_as_float((uint32_t)static_cast<const uint16_t *>(row)[i] << 16);
-    return (float)static_cast<const _Float16 *>(row)[i];
+static __device__ __forceinline__ uint32_t key_at(const char *row, int64_t i) {
+    if constexpr (DT == kF32) {
+        return key_f32(reinterpret_cast<const uint32_t *>(row)[i]);
+    } else {
+        return key_16<DT>(reinterpret_cast<const uint16_t *>(row)[i]);
+    }
+}
+// keys of entries i .. i + kVec - 1 (0 behind the row's end)
+template <int DT>
+static __device__ __forceinline__ void keys_at(const char *row, int64_t i, int64_t n, uint32_t (&k)[kVec<DT>]) {
+    if (i + kVec<DT> <= n) {
+        uint32_t w[4];
+        __builtin_memcpy(w, row + i * kBytes<DT>, 16);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) {
+            if constexpr (DT == kF32) {
+                k[e] = key_f32(w[e]);
+            } else {
+                k[e] = key_16<DT>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) k[e] = i + e < n ? key_at<DT>(row, i + e) : 0u;
+    }
 }
 
+// ---- weights ----------------------------------------------------------------------------------------------------
+// 2^y for y <= 0 by 2^n times the Taylor polynomial of 2^f, |f| <= 1/2: (ln 2 / 2)^13 / 13! = 2e-16.
+static __device__ __forceinline__ double pow2(double y) {
+    y = fmax(y, -1100.0);
+    const double n = rint(y), f = y - n;
+    constexpr double L = 0.69314718055994530941723212145818;
+    constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
+                     c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11,
+                     c12 = c11 * L / 12;
+    double p = fma(c12, f, c11);
+    p = fma(p, f, c10);
+    p = fma(p, f, c9);
+    p = fma(p, f, c8);
+    p = fma(p, f, c7);
+    p = fma(p, f, c6);
+    p = fma(p, f, c5);
+    p = fma(p, f, c4);
+    p = fma(p, f, c3);
+    p = fma(p, f, c2);
+    p = fma(p, f, c1);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+constexpr double kLog2e = 1.4426950408889634073599246810019;
+
+static __device__ __forceinline__ double reciprocal(double d) {   // d in [1, 2] (or a few times that)
+    double r = __builtin_amdgcn_rcp(d);
+    r = fma(fma(-d, r, 1.0), r, r);
+    return fma(fma(-d, r, 1.0), r, r);
+}
+// log(1 + z), z in [0, 1]: 2 atanh(s) with s = z / (2 + z) <= 1/3; (1/9)^16 / 33 = 2e-17
+static __device__ __forceinline__ double log1p_unit(double z) {
+    const double s = z * reciprocal(2.0 + z), q = s * s;
+    double p = 1.0 / 31;
+    p = fma(p, q, 1.0 / 29);
+    p = fma(p, q, 1.0 / 27);
+    p = fma(p, q, 1.0 / 25);
+    p = fma(p, q, 1.0 / 23);
+    p = fma(p, q, 1.0 / 21);
+    p = fma(p, q, 1.0 / 19);
+    p = fma(p, q, 1.0 / 17);
+    p = fma(p, q, 1.0 / 15);
+    p = fma(p, q, 1.0 / 13);
+    p = fma(p, q, 1.0 / 11);
+    p = fma(p, q, 1.0 / 9);
+    p = fma(p, q, 1.0 / 7);
+    p = fma(p, q, 1.0 / 5);
+    p = fma(p, q, 1.0 / 3);
+    return 2.0 * fma(p * q, s, s);
+}
 template <bool OPACITY>
 static __device__ __forceinline__ double log_weight(double x) {
     if constexpr (!OPACITY) return x;
-    return x < 0.0 ? x - log1p(exp(x)) : -log1p(exp(-x));
+    return fmin(x, 0.0) - log1p_unit(pow2(-fabs(x) * kLog2e));
 }
 
-template <bool OPACITY>
-static __device__ __forceinline__ double weight(uint32_t key, const SampleRow &s) {
-    if (key == s.max_key) return 1.0;          // (+inf - +inf)
-    return exp((log_weight<OPACITY>((double)value_of(key)) - s.l_max) * s.inv_t);
-}
-
-// ---- workgroup sums, 1024 threads; every thread gets the result; fixed order ------------------------------------
-static __device__ __forceinline__ double block_sum_d(double v, double *red /* [16] */) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double r = 0.0;
-    for (int w = 0; w < kSelThreads / 64; w++) r += red[w];
-    return r;
-}
-static __device__ __forceinline__ int64_t block_sum_i(int64_t v, double *red) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __longlong_as_double(v);
-    __syncthreads();
-    int64_t r = 0;
-    for (int w = 0; w < kSelThreads / 64; w++) r += __double_as_longlong(red[w]);
-    return r;
-}
-
-// One workgroup per row: maximum, threshold by bisection over the key's bits, running sums per 16 entries.
+// Weights relative to the key `top` (its own is 1).
+struct Scale {
+    double l_top, rate, norm;                  // rate = log2(e) / T;  norm = 1 / sigmoid(top)
+    uint32_t top;
+    bool unit;                                 // opacities at temperature 1: w = sigmoid(x) * norm
+};
 template <int DT, bool OPACITY>
-__global__ void __launch_bounds__(kSelThreads)
-k_sample_row(SampleArgs a, SampleRow *__restrict__ rows, double *__restrict__ seg_sum,
-             uint32_t *__restrict__ seg_ties) {
-    __shared__ double red[kSelThreads / 64];
-    __shared__ double wave_sum[kSelThreads / 64];
-    __shared__ uint32_t wave_tie[kSelThreads / 64];
+static __device__ __forceinline__ Scale scale_for(uint32_t top, double inv_t) {
+    Scale s;
+    const double x = (double)value_of<DT>(top);
+    s.top = top;
+    s.l_top = log_weight<OPACITY>(x);
+    s.rate = inv_t * kLog2e;
+    s.unit = OPACITY && inv_t == 1.0 && x > -700.0;
+    s.norm = s.unit ? 1.0 + exp(-x) : 1.0;
+    return s;
+}
+template <int DT, bool OPACITY>
+static __device__ __forceinline__ double weight(uint32_t key, const Scale &s) {
+    if (key == s.top) return 1.0;              // (also +inf - +inf)
+    const double x = (double)value_of<DT>(key);
+    if constexpr (OPACITY) {
+        if (s.unit) {
+            const double z = pow2(-fabs(x) * kLog2e);
+            return fmin((x < 0.0 ? z : 1.0) * reciprocal(1.0 + z) * s.norm, 1.0);
+        }
+    }
+    return pow2((log_weight<OPACITY>(x) - s.l_top) * s.rate);
+}
+// ---- digits of a threshold ----------------------------------------------------------------------------------------
+constexpr int kBins = 2048;
+template <int DT>
+constexpr int kUsedLevels = DT == kF32 ? 3 : 2;   // a 16-bit type's key ends within the second digit
+static __device__ __forceinline__ int digit_shift(int level) { return level == 0 ? 21 : (level == 1 ? 10 : 0); }
+static __device__ __forceinline__ uint32_t digit_of(uint32_t key, int level) {
+    return level == 0 ? key >> 21 : (level == 1 ? (key >> 10) & 2047u : key & 1023u);
+}
+// the digits above `level` of `key` are those found
+static __device__ __forceinline__ bool agrees(uint32_t key, uint32_t found, int level) {
+    return level == 0 || (key >> (level == 1 ? 21 : 10)) == (found >> (level == 1 ? 21 : 10));
+}
+
+// One search, for top-k (counts) or top-p (masses), as it stands between two digits.
+struct Search {
+    uint64_t above;                            // count or mass over the digits found
+    double goal;                               // count or mass to reach
+    uint32_t found;
+    uint32_t done;                             // nothing to cut: every candidate is kept
+};
+
+// w * unit <= 2^50, rounded to the nearest integer: the low bits of that number plus 2^52
+static __device__ __forceinline__ uint64_t fixed(double w, double unit) {
+    return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) - 0x4330000000000000ull;
+}
+
+// Exclusive scan over the workgroup in thread order, THREADS a multiple of 64; `total` gets the sum.
+template <int THREADS, typename T>
+static __device__ __forceinline__ T block_scan(T v, T *wave_sums /* LDS [THREADS / 64] */, T &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T s = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const T o = __shfl_up(s, off, 64);
+        if (lane >= off) s += o;
+    }
+    T before = __shfl_up(s, 1, 64);
+    if (lane == 0) before = T(0);
+    if constexpr (THREADS == 64) {
+        total = __shfl(s, 63, 64);
+        return before;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sums[wave] = s;
+    __syncthreads();
+    T base = T(0), all = T(0);
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        if (w == wave) base = all;
+        all += wave_sums[w];
+    }
+    total = all;
+    return base + before;
+}
+
+// The digit in which the running total, from the largest digit down, reaches the goal.  `bin(i)`: count or mass of digit
+// i.  Every thread of the workgroup gets the digit and what lies above it; called with the histogram complete.
+struct Picked {
+    uint32_t digit;
+    uint64_t above, total;
+};
+template <int THREADS, typename F>
+static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goal_is_share, double share,
+                                    uint64_t *wave_sums, Picked *out /* LDS */) {
+    constexpr int per = kBins / THREADS < 1 ? 1 : kBins / THREADS;
+    const int tid = threadIdx.x, high = kBins - 1 - tid * per;
+    uint64_t mine = 0;
+#pragma unroll 4
+    for (int j = 0; j < per; j++) mine += bin(high - j);
+    uint64_t total;
+    uint64_t run = above + block_scan<THREADS>(mine, wave_sums, total);
+    const double need = goal_is_share ? share * (double)total : goal;
+    if (tid == 0) *out = {kBins, 0, total};
+    __syncthreads();
+    // the first thread whose part crosses: its start is below the goal, its end is not
+    if ((double)run < need && (double)(run + mine) >= need && mine > 0) {
+        for (int j = 0; j < per; j++) {
+            const uint64_t b = bin(high - j);
+            if (b > 0 && (double)(run + b) >= need) {
+                *out = {(uint32_t)(high - j), run, total};
+                break;
+            }
+            run += b;
+        }
+    }
+    __syncthreads();
+    const Picked p = *out;
+    __syncthreads();
+    return p;
+}
+
+static __device__ __forceinline__ uint32_t ties_for(uint64_t above, double goal, double tie_weight, double unit,
+                                                    uint64_t have) {
+    const double w = (double)fixed(tie_weight, unit);
+    const double n = w > 0.0 ? ceil((goal - (double)above) / w) : (double)have;
+    return (uint32_t)fmin(fmax(n, 1.0), (double)have);
+}
+
+// floor(u * total), below total: the running sums that exceed u * total are those that exceed it
+static __device__ __forceinline__ uint64_t goal_of(float u, uint64_t total) {
+    const double g = fmax((double)u, 0.0) * (double)total;
+    return g < (double)total ? min((uint64_t)g, total - 1) : total - 1;
+}
+
+// ---- rows of up to 8192 entries ------------------------------------------------------------------------------------
+constexpr int kEach = 8;                       // entries per thread
+
+// One workgroup per row; thread t holds entries 8 t .. 8 t + 7, so that thread order is index order.  Bound by latency: a
+// dozen barriers, and per digit one LDS atomic an entry; the entries are read once.
+template <int DT, bool OPACITY, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+    __shared__ uint64_t kept_w[kEach][THREADS + 1];   // weight of entry 8 t + e at [e][t]; 0: not kept
+    __shared__ uint64_t run_sum[THREADS];
+    __shared__ uint64_t mass[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ uint64_t waves_u[THREADS / 64];
+    __shared__ uint32_t waves_i[THREADS / 64];
+    __shared__ Picked pick;
     const int r = blockIdx.x, tid = threadIdx.x, n = a.cols;
-    const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * (DT == kF32 ? 4 : 2);
+    const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
     const RowSettings set = row_settings(a, r);
-    auto key_at = [&](int64_t i) { return key_of(load_value<DT>(row, i)); };
 
+    uint32_t key[kEach];
+#pragma unroll
+    for (int q = 0; q < kEach / kVec<DT>; q++) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, (int64_t)tid * kEach + q * kVec<DT>, n, k);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
+    }
     uint32_t mx = 0;
-    for (int64_t i = tid; i < n; i += kSelThreads) mx = max(mx, key_at(i));
+#pragma unroll
+    for (int e = 0; e < kEach; e++) mx = max(mx, key[e]);
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
-    if ((tid & 63) == 0) wave_tie[tid >> 6] = mx;
+    if constexpr (THREADS > 64) {
+        if ((tid & 63) == 0) waves_i[tid >> 6] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) mx = max(mx, waves_i[w]);
+    }
+    if (!set.ok || mx == 0) {
+        for (int j = tid; j < a.draws; j += THREADS) ids[(size_t)r * a.draws + j] = -1;
+        return;
+    }
+    const Scale s = scale_for<DT, OPACITY>(mx, set.inv_t);
+    double w[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        w[e] = 0.0;
+        if (key[e] != 0 && (!set.greedy || key[e] == mx)) w[e] = weight<DT, OPACITY>(key[e], s);
+    }
+    uint32_t thr = 0, ties = 0;
+    if (!set.greedy && set.top_k > 0) {
+        Search f = {0, (double)set.top_k, 0, 0};
+        for (int level = 0; level < kUsedLevels<DT> && !f.done; level++) {
+            for (int b = tid; b < kBins; b += THREADS) count[b] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                if (key[e] != 0 && agrees(key[e], f.found, level)) atomicAdd(&count[digit_of(key[e], level)], 1u);
+            __syncthreads();
+            const Picked p = pick_digit<THREADS>([&](int i) { return (uint64_t)count[i]; }, f.above, f.goal, false, 0.0,
+                                                 waves_u, &pick);
+            if (p.digit == kBins) f.done = 1;  // fewer candidates than k
+            else f.found |= p.digit << digit_shift(level);
+            f.above = p.above;
+        }
+        if (!f.done) {
+            thr = f.found;
+            ties = (uint32_t)set.top_k - (uint32_t)f.above;
+        }
+    }
+    if (!set.greedy && set.top_p < 1.0) {
+        const uint32_t kthr = thr, kties = ties;
+        double kw = 0.0;
+        if (kthr) kw = weight<DT, OPACITY>(kthr, s);
+        Search f = {0, 0.0, 0, 0};
+        uint64_t have = 0;
+        for (int level = 0; level < kUsedLevels<DT>; level++) {
+            for (int b = tid; b < kBins; b += THREADS) {
+                mass[b] = 0;
+                count[b] = 0;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                if (key[e] > kthr && agrees(key[e], f.found, level)) {
+                    const uint32_t d = digit_of(key[e], level);
+                    atomicAdd((unsigned long long *)&mass[d], (unsigned long long)fixed(w[e], a.unit));
+                    if (level == kUsedLevels<DT> - 1) atomicAdd(&count[d], 1u);
+                }
+            __syncthreads();
+            if (tid == 0 && kthr && agrees(kthr, f.found, level)) {   // the ties that top-k left, as one
+                const uint32_t d = digit_of(kthr, level);
+                mass[d] += (uint64_t)kties * fixed(kw, a.unit);
+                count[d] += kties;
+            }
+            __syncthreads();
+            const Picked p = pick_digit<THREADS>([&](int i) { return mass[i]; }, f.above, f.goal, level == 0, set.top_p,
+                                                 waves_u, &pick);
+            if (level == 0) f.goal = set.top_p * (double)p.total;
+            if (p.digit == kBins) {            // (nothing weighs anything in fixed point but the first)
+                f.done = 1;
+                break;
+            }
+            f.found |= p.digit << digit_shift(level);
+            f.above = p.above;
+            have = count[p.digit];
+            __syncthreads();
+        }
+        if (!f.done) {
+            thr = f.found;
+            ties = ties_for(f.above, f.goal, weight<DT, OPACITY>(thr, s), a.unit, have);
+        }
+    }
+    // what is kept: ties by their rank in index order
+    uint32_t rank = 0;
+    if (thr) {
+        uint32_t mine = 0, all;
+#pragma unroll
+        for (int e = 0; e < kEach; e++) mine += key[e] == thr;
+        rank = block_scan<THREADS>(mine, waves_i, all);
+    }
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const bool tied = thr != 0 && key[e] == thr;
+        const bool keep = key[e] > thr || (tied && rank < ties);
+        rank += tied;
+        const uint64_t v = (keep && w[e] >= set.min_p) ? fixed(w[e], a.unit) : 0ull;
+        kept_w[e][tid] = v;
+        sum += v;
+    }
+    uint64_t total;
+    run_sum[tid] = block_scan<THREADS>(sum, waves_u, total);
     __syncthreads();
-    for (int w = 0; w < kSelThreads / 64; w++) mx = max(mx, wave_tie[w]);
-    __syncthreads();
-
-    SampleRow s;
-    s.max_key = mx;
-    s.inv_t = 1.0 / set.temperature;
-    s.l_max = log_weight<OPACITY>((double)value_of(mx));
-    s.min_p = set.min_p;
-    s.threshold = 0;
-    s.ties = 0;
-    s.total = 0.0;
-    s.pad = 0;
-    const bool any = set.ok && mx != 0;
-    auto count_from = [&](uint32_t t) {
-        int64_t c = 0;
-        for (int64_t i = tid; i < n; i += kSelThreads) c += key_at(i) >= t;
-        return block_sum_i(c, red);
-    };
-    auto mass_from = [&](uint32_t t) {
-        double m = 0.0;
-        for (int64_t i = tid; i < n; i += kSelThreads) {
-            const uint32_t k = key_at(i);
-            if (k >= t) m += weight<OPACITY>(k, s);
+    for (int j = tid; j < a.draws; j += THREADS) {
+        const float u = uniforms[(size_t)r * a.draws + j];
+        const uint64_t goal = set.greedy ? 0ull : goal_of(u, total);
+        int lo = 0, hi = THREADS;              // run_sum[lo] <= goal < run_sum[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (run_sum[mid] <= goal) lo = mid;
+            else hi = mid;
         }
-        return block_sum_d(m, red);
-    };
-    if (any && set.top_k < n && count_from(1u) > set.top_k) {
-        uint32_t t = 0;                        // largest key with at least top_k entries from it on
-        for (int b = 31; b >= 0; b--)
-            if (count_from(t | (1u << b)) >= set.top_k) t |= 1u << b;
-        s.threshold = t;
-        s.ties = (uint32_t)(set.top_k - (t == 0xFFFFFFFFu ? 0 : count_from(t + 1u)));
+        uint64_t c = run_sum[lo];
+        int e = -1;
+        do c += kept_w[++e][lo];
+        while (c <= goal && e < kEach - 1);
+        ids[(size_t)r * a.draws + j] = isnan(u) ? -1 : lo * kEach + e;
     }
-    if (any && set.top_p < 1.0) {
-        const uint32_t kt = s.threshold;
-        const double tie_mass = kt ? (double)s.ties * weight<OPACITY>(kt, s) : 0.0;
-        const double goal = set.top_p * (mass_from(kt + 1u) + tie_mass);
-        uint32_t t = 0;                        // largest key with mass >= goal from it on, inside the first k
-        for (int b = 31; b >= 0; b--) {
-            const uint32_t c = t | (1u << b);
-            if (c <= kt || mass_from(c) >= goal) t = c;
-        }
-        if (t > kt) {
-            const double above = t == 0xFFFFFFFFu ? 0.0 : mass_from(t + 1u), w = weight<OPACITY>(t, s);
-            const int64_t have = count_from(t) - (t == 0xFFFFFFFFu ? 0 : count_from(t + 1u));
-            int64_t c = w > 0.0 ? (int64_t)fmin(ceil((goal - above) / w), (double)have) : have;
-            s.threshold = t;
-            s.ties = (uint32_t)max(c, (int64_t)1);
-        } else if (kt) {                       // the border lies among the ties that top-k left
-            const double above = mass_from(kt + 1u), w = weight<OPACITY>(kt, s);
-            const double c = w > 0.0 ? ceil((goal - above) / w) : (double)s.ties;
-            s.ties = (uint32_t)fmin(fmax(c, 1.0), (double)s.ties);
-        }
-    }
-
-    // running sums in index order
-    double base = 0.0;
-    uint32_t tie_base = 0;
-    const int64_t nseg = (n + kSeg - 1) / kSeg;
-    double *out_sum = seg_sum + (size_t)r * nseg;
-    uint32_t *out_tie = seg_ties + (size_t)r * nseg;
-    for (int64_t first = 0; any && first < n; first += kSelChunk) {
-        const int64_t i0 = first + (int64_t)tid * kSeg, i1 = min(i0 + kSeg, (int64_t)n);
-        uint32_t tie = 0;
-        for (int64_t i = i0; i < i1; i++) tie += s.threshold != 0 && key_at(i) == s.threshold;
-        // exclusive scans over the workgroup: ties first, they decide what the sums hold
-        uint32_t ti = tie;
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)ti, off, 64);
-            if ((tid & 63) >= off) ti += o;
-        }
-        __syncthreads();
-        if ((tid & 63) == 63) wave_tie[tid >> 6] = ti;
-        __syncthreads();
-        uint32_t before = tie_base + ti - tie, all_ties = 0;
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w < (tid >> 6)) before += wave_tie[w];
-            all_ties += wave_tie[w];
-        }
-        double sum = 0.0;
-        uint32_t rank = before;
-        for (int64_t i = i0; i < i1; i++) {
-            const uint32_t k = key_at(i);
-            const bool tied = s.threshold != 0 && k == s.threshold;
-            const bool kept = k > s.threshold || (tied && rank < s.ties);
-            rank += tied;
-            if (!kept) continue;
-            const double w = weight<OPACITY>(k, s);
-            if (w >= s.min_p) sum += w;
-        }
-        double inc = sum;
-        for (int off = 1; off < 64; off <<= 1) {
-            const double o = __shfl_up(inc, off, 64);
-            if ((tid & 63) >= off) inc += o;
-        }
-        __syncthreads();
-        if ((tid & 63) == 63) wave_sum[tid >> 6] = inc;
-        __syncthreads();
-        double pre = 0.0, chunk = 0.0;
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w == (tid >> 6)) pre = chunk;
-            chunk += wave_sum[w];
-        }
-        if (i0 < n) {
-            const double excl = __shfl_up(inc, 1, 64);
-            out_sum[i0 / kSeg] = base + (pre + ((tid & 63) ? excl : 0.0));
-            out_tie[i0 / kSeg] = before;
-        }
-        base += chunk;
-        tie_base += all_ties;
-    }
-    s.total = any ? base : 0.0;
-    if (tid == 0) rows[r] = s;
 }
 
-// One thread per draw: the last segment whose running sum does not exceed the goal, then its entries one by one.
-template <int DT, bool OPACITY>
+// ---- longer rows ------------------------------------------------------------------------------------------------------
+constexpr int kSeg = 16;                       // entries one thread sums: the grain of the stored running sums
+constexpr int kChunkThreads = 256;
+constexpr int kChunk = kChunkThreads * kSeg;
+constexpr int kHistThreads = 1024;
+
+// A row's state between the launches.
+struct LongRow {
+    double inv_t, top_p, min_p;
+    uint64_t total, tie_weight;
+    Search k, p;
+    uint32_t max_key, thr, ties, arrived;
+    int32_t top_k;
+    uint32_t ok, greedy, pad;
+};
+
+struct LongArgs {
+    LongRow *rows;
+    uint64_t *mass;                            // [rows][kBins]
+    uint32_t *count;                           // [rows][kBins]
+    uint32_t *chunk_max;                       // [rows][chunks]
+    uint64_t *chunk_sum;                       // [rows][chunks]: sums, then running sums
+    uint32_t *chunk_ties;                      // [rows][chunks]: ties, then running ties
+    uint64_t *seg_sum;                           // [rows][chunks][256] running sums inside the chunk
+    uint32_t *seg_ties;                        // [rows][chunks][256]
+    int chunks;
+};
+
+template <int DT>
+static __device__ __forceinline__ const char *row_base(const SampleArgs &a, int r) {
+    return static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kChunkThreads)
+k_long_max(SampleArgs a, LongArgs g) {
+    __shared__ uint32_t waves[kChunkThreads / 64];
+    const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
+    const char *row = row_base<DT>(a, r);
+    uint32_t mx = 0;
+#pragma unroll
+    for (int q = 0; q < kSeg / kVec<DT>; q++) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, (int64_t)c * kChunk + ((int64_t)q * kChunkThreads + tid) * kVec<DT>, a.cols, k);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) mx = max(mx, k[e]);
+    }
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+    if ((tid & 63) == 0) waves[tid >> 6] = mx;
+    __syncthreads();
+    if (tid == 0) g.chunk_max[(size_t)r * g.chunks + c] = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+}
+
+// The row's settings and maximum, nothing cut yet.
+static __device__ __forceinline__ LongRow long_row(const SampleArgs &a, int r, uint32_t max_key) {
+    const RowSettings set = row_settings(a, r);
+    LongRow s = {};
+    s.inv_t = set.inv_t;
+    s.top_p = set.top_p;
+    s.min_p = set.min_p;
+    s.top_k = set.top_k;
+    s.ok = set.ok && max_key != 0;
+    s.greedy = set.greedy;
+    s.max_key = max_key;
+    s.k.goal = (double)set.top_k;
+    s.k.done = set.greedy || !s.ok || set.top_k == 0;
+    s.p.done = set.greedy || !s.ok || !(set.top_p < 1.0);
+    return s;
+}
+
+// Maximum over the row's chunks, by every workgroup for itself.
+template <int THREADS>
+static __device__ __forceinline__ uint32_t row_max(const LongArgs &g, int r, uint32_t *waves /* LDS [THREADS / 64] */) {
+    uint32_t mx = 0;
+    for (int c = threadIdx.x; c < g.chunks; c += THREADS) mx = max(mx, g.chunk_max[(size_t)r * g.chunks + c]);
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) mx = max(mx, waves[w]);
+    __syncthreads();
+    return mx;
+}
+
+// One workgroup per row: its state, empty histograms.
+__global__ void __launch_bounds__(kHistThreads)
+k_long_begin(SampleArgs a, LongArgs g, int histograms) {
+    __shared__ uint32_t waves[kHistThreads / 64];
+    const int r = blockIdx.x, tid = threadIdx.x;
+    if (histograms)
+        for (int b = tid; b < kBins; b += kHistThreads) {
+            g.mass[(size_t)r * kBins + b] = 0;
+            g.count[(size_t)r * kBins + b] = 0;
+        }
+    const uint32_t mx = row_max<kHistThreads>(g, r, waves);
+    if (tid == 0) g.rows[r] = long_row(a, r, mx);
+}
+
+// A digit of the top-k threshold (MASS false) or of the top-p threshold.  `parts` workgroups per row; each adds its
+// part's histogram to the row's, and the last of them to arrive picks the digit and empties the row's histogram again.
+// The row's counters are only touched by device-wide atomics here: the caches of the eight dies do not see each other's
+// plain stores within a launch.
+template <int DT, bool OPACITY, bool MASS>
+__global__ void __launch_bounds__(kHistThreads)
+k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
+    __shared__ uint64_t mass[MASS ? kBins : 1];
+    __shared__ uint32_t count[kBins];
+    __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ Picked pick;
+    __shared__ uint32_t last;
+    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
+    LongRow &st = g.rows[r];
+    const Search f = MASS ? st.p : st.k;
+    if (f.done) return;
+    const bool final_level = level == kUsedLevels<DT> - 1;
+    const uint32_t kthr = MASS ? st.thr : 0u, kties = MASS ? st.ties : 0u;
+    const Scale s = scale_for<DT, OPACITY>(st.max_key, st.inv_t);
+    for (int b = tid; b < kBins; b += kHistThreads) {
+        if constexpr (MASS) mass[b] = 0;
+        count[b] = 0;
+    }
+    __syncthreads();
+    const char *row = row_base<DT>(a, r);
+    const int64_t n = a.cols;
+    for (int64_t i = ((int64_t)part * kHistThreads + tid) * kVec<DT>; i < n; i += (int64_t)parts * kHistThreads * kVec<DT>) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, i, n, k);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) {
+            if (!(k[e] > kthr) || !agrees(k[e], f.found, level)) continue;
+            const uint32_t d = digit_of(k[e], level);
+            if constexpr (MASS) {
+                atomicAdd((unsigned long long *)&mass[d],
+                          (unsigned long long)fixed(weight<DT, OPACITY>(k[e], s), a.unit));
+                if (final_level) atomicAdd(&count[d], 1u);
+            } else {
+                atomicAdd(&count[d], 1u);
+            }
+        }
+    }
+    __syncthreads();
+    uint64_t *row_mass = g.mass + (size_t)r * kBins;
+    uint32_t *row_count = g.count + (size_t)r * kBins;
+    for (int b = tid; b < kBins; b += kHistThreads) {
+        if constexpr (MASS)
+            if (mass[b]) atomicAdd((unsigned long long *)&row_mass[b], (unsigned long long)mass[b]);
+        if (count[b]) atomicAdd(&row_count[b], count[b]);
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = __hip_atomic_fetch_add(&st.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int b = tid; b < kBins; b += kHistThreads) {
+        if constexpr (MASS) {
+            mass[b] = __hip_atomic_load(&row_mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&row_mass[b], (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        count[b] = __hip_atomic_load(&row_count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&row_count[b], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (MASS && tid == 0 && kthr && agrees(kthr, f.found, level)) {   // the ties that top-k left, as one
+        const uint32_t d = digit_of(kthr, level);
+        mass[MASS ? d : 0] += (uint64_t)kties * fixed(weight<DT, OPACITY>(kthr, s), a.unit);
+        count[d] += kties;
+    }
+    __syncthreads();
+    const Picked p = pick_digit<kHistThreads>([&](int i) { return MASS ? mass[MASS ? i : 0] : (uint64_t)count[i]; }, f.above,
+                                              f.goal, MASS && level == 0, st.top_p, waves_u, &pick);
+    if (tid == 0) {
+        Search next = f;
+        if (MASS && level == 0) next.goal = st.top_p * (double)p.total;
+        if (p.digit == kBins) {
+            next.done = 1;
+        } else {
+            next.found |= p.digit << digit_shift(level);
+            next.above = p.above;
+            if (final_level) {
+                st.thr = next.found;
+                st.ties = MASS ? ties_for(next.above, next.goal, weight<DT, OPACITY>(next.found, s), a.unit, count[p.digit])
+                               : (uint32_t)st.top_k - (uint32_t)next.above;
+            }
+        }
+        if (MASS) st.p = next;
+        else st.k = next;
+        st.arrived = 0;
+    }
+}
+
+// Per chunk: running sums of the kept weights and of the ties per 16 entries, and their totals.  CUT false: no row has a
+// threshold, and (BEGUN false) no launch has prepared the rows' state: the row's maximum is taken from its chunks' here.
+template <int DT, bool OPACITY, bool CUT, bool BEGUN>
+__global__ void __launch_bounds__(kChunkThreads)
+k_long_sums(SampleArgs a, LongArgs g) {
+    __shared__ uint64_t waves_u[kChunkThreads / 64];
+    __shared__ uint32_t waves_i[kChunkThreads / 64];
+    const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
+    const char *row = row_base<DT>(a, r);
+    const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * kSeg;
+    uint32_t key[kSeg];
+#pragma unroll
+    for (int q = 0; q < kSeg / kVec<DT>; q++) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
+    }
+    uint32_t top, thr = 0;
+    double inv_t, min_p;
+    bool greedy, ok;
+    if constexpr (BEGUN) {
+        const LongRow &st = g.rows[r];
+        top = st.max_key;
+        thr = CUT ? st.thr : 0u;
+        inv_t = st.inv_t;
+        min_p = st.min_p;
+        greedy = st.greedy;
+        ok = st.ok;
+    } else {
+        top = row_max<kChunkThreads>(g, r, waves_i);
+        const LongRow st = long_row(a, r, top);
+        inv_t = st.inv_t;
+        min_p = st.min_p;
+        greedy = st.greedy;
+        ok = st.ok;
+        if (c == 0 && tid == 0) g.rows[r] = st;
+    }
+    const Scale s = scale_for<DT, OPACITY>(top, inv_t);
+    uint64_t sum = 0;
+    uint32_t ties = 0;
+    if (ok) {
+#pragma unroll
+        for (int e = 0; e < kSeg; e++) {
+            if (CUT && thr) ties += key[e] == thr;
+            if (!(key[e] > thr) || (greedy && key[e] != top)) continue;
+            const double w = weight<DT, OPACITY>(key[e], s);
+            if (w >= min_p) sum += fixed(w, a.unit);
+        }
+    }
+    const size_t at = (size_t)r * g.chunks + c;
+    const size_t seg = at * kChunkThreads + tid;
+    uint64_t total;
+    g.seg_sum[seg] = block_scan<kChunkThreads>(sum, waves_u, total);
+    if (tid == 0) g.chunk_sum[at] = total;
+    if constexpr (CUT) {
+        uint32_t all = 0, ties_before = 0;
+        if (thr) ties_before = block_scan<kChunkThreads>(ties, waves_i, all);
+        g.seg_ties[seg] = ties_before;
+        if (tid == 0) g.chunk_ties[at] = all;
+    }
+}
+
+// One workgroup per row: running sums over the chunks.
+template <int DT, bool OPACITY, bool CUT>
+__global__ void __launch_bounds__(kHistThreads)
+k_long_scan(SampleArgs a, LongArgs g) {
+    __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ uint32_t waves_i[kHistThreads / 64];
+    const int r = blockIdx.x, tid = threadIdx.x;
+    LongRow &st = g.rows[r];
+    const size_t first = (size_t)r * g.chunks;
+    const bool ok = st.ok;
+    uint32_t thr = 0, ties = 0;
+    uint64_t tie_weight = 0;
+    if constexpr (CUT) {
+        thr = st.thr;
+        ties = st.ties;
+        if (thr) {
+            const double w = weight<DT, OPACITY>(thr, scale_for<DT, OPACITY>(st.max_key, st.inv_t));
+            tie_weight = w >= st.min_p ? fixed(w, a.unit) : 0ull;
+        }
+    }
+    uint64_t base = 0;
+    uint32_t tie_base = 0;
+    for (int c0 = 0; c0 < g.chunks; c0 += kHistThreads) {
+        const int c = c0 + tid;
+        const bool in = c < g.chunks;
+        uint64_t v = in ? g.chunk_sum[first + c] : 0ull;
+        if (CUT && thr) {
+            const uint32_t here = in ? g.chunk_ties[first + c] : 0u;
+            uint32_t all;
+            const uint32_t before = tie_base + block_scan<kHistThreads>(here, waves_i, all);
+            tie_base += all;
+            if (in) g.chunk_ties[first + c] = before;
+            v += tie_weight * min(ties > before ? ties - before : 0u, here);
+        }
+        uint64_t all;
+        const uint64_t before = base + block_scan<kHistThreads>(v, waves_u, all);
+        base += all;
+        if (in) g.chunk_sum[first + c] = before;
+    }
+    if (tid == 0) {
+        st.total = ok ? base : 0ull;
+        st.tie_weight = tie_weight;
+    }
+}
+
+// One thread per draw: the last chunk, then the last 16 entries, whose running sum does not exceed the goal, then entry by
+// entry.  (Integer sums: what is found there holds a weight.)
+template <int DT, bool OPACITY, bool CUT>
 __global__ void __launch_bounds__(256)
-k_sample_draw(SampleArgs a, const SampleRow *__restrict__ rows, const double *__restrict__ seg_sum,
-              const uint32_t *__restrict__ seg_ties, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+k_long_draw(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
     const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (at >= (int64_t)a.rows * a.draws) return;
-    const int r = (int)(at / a.draws), n = a.cols;
-    const SampleRow s = rows[r];
+    const int r = (int)(at / a.draws);
+    const LongRow &st = g.rows[r];
+    const uint64_t total = st.total;
     const float u = uniforms[at];
-    if (!(s.total > 0.0) || isnan(u)) {
+    if (total == 0 || isnan(u)) {
         ids[at] = -1;
         return;
     }
-    double goal = (double)u * s.total;
-    if (goal < 0.0) goal = 0.0;
-    if (goal >= s.total) goal = s.total * (1.0 - 0x1p-53);
-    const int64_t nseg = ((int64_t)n + kSeg - 1) / kSeg;
-    const double *sums = seg_sum + (size_t)r * nseg;
-    int64_t lo = 0, hi = nseg;                 // sums[lo] <= goal < sums[hi]
+    const bool greedy = st.greedy;
+    const uint64_t goal = greedy ? 0ull : goal_of(u, total);
+    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
+    int lo = 0, hi = g.chunks;                 // chunk_sum[lo] <= goal < chunk_sum[hi]
     while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (sums[mid] <= goal) lo = mid;
+        const int mid = lo + ((hi - lo) >> 1);
+        if (chunk_sum[mid] <= goal) lo = mid;
         else hi = mid;
     }
-    const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * (DT == kF32 ? 4 : 2);
-    double c = sums[lo];
-    uint32_t rank = seg_ties[(size_t)r * nseg + lo];
+    const size_t c = (size_t)r * g.chunks + lo;
+    const uint64_t rest = goal - g.chunk_sum[c];
+    uint64_t tie_weight = 0;
+    uint32_t thr = 0, left = 0;                // ties of this chunk that are kept
+    if constexpr (CUT) {
+        thr = st.thr;
+        if (thr) {
+            tie_weight = st.tie_weight;
+            const uint32_t before = g.chunk_ties[c];
+            left = st.ties > before ? st.ties - before : 0u;
+        }
+    }
+    const uint64_t *seg_sum = g.seg_sum + c * kChunkThreads;
+    const uint32_t *seg_ties = CUT ? g.seg_ties + c * kChunkThreads : nullptr;
+    auto sum_before = [&](int i) {
+        uint64_t v = seg_sum[i];
+        if (CUT && thr) v += tie_weight * min(left, seg_ties[i]);
+        return v;
+    };
+    int sl = 0, sh = kChunkThreads;
+    while (sh - sl > 1) {
+        const int mid = (sl + sh) >> 1;
+        if (sum_before(mid) <= rest) sl = mid;
+        else sh = mid;
+    }
+    uint64_t run = sum_before(sl);
+    uint32_t rank = (CUT && thr) ? seg_ties[sl] : 0u;
+    const char *row = row_base<DT>(a, r);
+    const int64_t i0 = (int64_t)lo * kChunk + (int64_t)sl * kSeg;
+    const uint32_t top = st.max_key;
+    const Scale s = scale_for<DT, OPACITY>(top, st.inv_t);
+    const double min_p = st.min_p;
     int64_t id = -1;
-    const int64_t i1 = min((lo + 1) * kSeg, (int64_t)n);
-    for (int64_t i = lo * kSeg; i < i1; i++) {
-        const uint32_t k = key_of(load_value<DT>(row, i));
-        const bool tied = s.threshold != 0 && k == s.threshold;
-        const bool kept = k > s.threshold || (tied && rank < s.ties);
-        rank += tied;
-        if (!kept) continue;
-        const double w = weight<OPACITY>(k, s);
-        if (!(w >= s.min_p) || !(w > 0.0)) continue;
-        c += w;
-        id = i;                                // (rounding of the last sum: the last entry that can be drawn)
-        if (c > goal) break;
+#pragma unroll
+    for (int q = 0; q < kSeg / kVec<DT>; q++) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
+        for (int e = 0; e < kVec<DT>; e++) {
+            const bool tied = CUT && thr != 0 && k[e] == thr;
+            const bool keep = k[e] > thr || (tied && rank < left);
+            rank += tied;
+            if (id >= 0 || !keep || (greedy && k[e] != top)) continue;
+            const double w = weight<DT, OPACITY>(k[e], s);
+            if (w >= min_p) run += fixed(w, a.unit);
+            if (run > rest) id = i0 + q * kVec<DT> + e;
+        }
     }
     ids[at] = (int32_t)id;
 }
 
+// ---- host -------------------------------------------------------------------------------------------------------------
+constexpr int kRowLimit = 8192;                // longest row of the one-workgroup form
+
 struct SampleLayout {
-    size_t rows_off, sum_off, tie_off, total;
-    SampleLayout(int rows, int cols) {
+    size_t rows, mass, count, chunk_max, chunk_sum, chunk_ties, seg_sum, seg_ties, total;
+    int chunks;
+    SampleLayout(int n_rows, int cols) {
         size_t o = 0;
         auto take = [&](size_t bytes) { size_t r = o; o += (bytes + 255) & ~(size_t)255; return r; };
-        const size_t nseg = ((size_t)cols + kSeg - 1) / kSeg;
-        rows_off = take((size_t)rows * sizeof(SampleRow));
-        sum_off = take((size_t)rows * nseg * sizeof(double));
-        tie_off = take((size_t)rows * nseg * sizeof(uint32_t));
-        total = o;
+        chunks = cols > kRowLimit ? (int)(((int64_t)cols + kChunk - 1) / kChunk) : 0;
+        const size_t n = (size_t)n_rows * chunks, some = chunks ? (size_t)n_rows : 0;
+        rows = take(some * sizeof(LongRow));
+        mass = take(some * kBins * 8);
+        count = take(some * kBins * 4);
+        chunk_max = take(n * 4);
+        chunk_sum = take(n * 8);
+        chunk_ties = take(n * 4);
+        seg_sum = take(n * kChunkThreads * 8);
+        seg_ties = take(n * kChunkThreads * 4);
+        total = o > 0 ? o : 256;
     }
 };
 
 template <int DT, bool OPACITY>
-static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *ids, char *ws, const SampleLayout &L,
-                         hipStream_t s) {
-    SampleRow *rows = (SampleRow *)(ws + L.rows_off);
-    double *sums = (double *)(ws + L.sum_off);
-    uint32_t *ties = (uint32_t *)(ws + L.tie_off);
-    GS_LAUNCH((k_sample_row<DT, OPACITY>), dim3(a.rows), dim3(kSelThreads), 0, s, a, rows, sums, ties);
-    GS_LAUNCH_CHECK();
-    const int64_t want = ((int64_t)a.rows * a.draws + 255) / 256;
-    GS_LAUNCH((k_sample_draw<DT, OPACITY>), dim3((unsigned)want), dim3(256), 0, s, a, rows, sums, ties, uniforms, ids);
+static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids, hipStream_t s) {
+    const dim3 grid(a.rows);
+    if (a.cols <= 64 * kEach) {
+        GS_LAUNCH((k_sample_row<DT, OPACITY, 64>), grid, dim3(64), 0, s, a, uniforms, ids);
+    } else if (a.cols <= 256 * kEach) {
+        GS_LAUNCH((k_sample_row<DT, OPACITY, 256>), grid, dim3(256), 0, s, a, uniforms, ids);
+    } else {
+        GS_LAUNCH((k_sample_row<DT, OPACITY, 1024>), grid, dim3(1024), 0, s, a, uniforms, ids);
+    }
     GS_LAUNCH_CHECK();
     return GS_OK;
+}
+
+// Up to this many chunks (16 M entries) k_long_sums reads the chunks' maxima itself, a few loads a thread; beyond, that
+// would grow with the square of the row.
+constexpr int kOwnMaxChunks = 4096;
+
+template <int DT, bool OPACITY, bool CUT>
+static int launch_long(const SampleArgs &a, const LongArgs &g, const float *uniforms, int32_t *ids, hipStream_t s) {
+    const dim3 chunks((unsigned)((int64_t)a.rows * g.chunks)), rows(a.rows);
+    GS_LAUNCH((k_long_max<DT>), chunks, dim3(kChunkThreads), 0, s, a, g);
+    GS_LAUNCH_CHECK();
+    const bool begun = CUT || g.chunks > kOwnMaxChunks;
+    if (begun) {
+        GS_LAUNCH(k_long_begin, rows, dim3(kHistThreads), 0, s, a, g, CUT ? 1 : 0);
+        GS_LAUNCH_CHECK();
+    }
+    if constexpr (CUT) {
+        // two workgroups per compute unit over all the rows, and no part of a row below its first 8192 entries
+        const int64_t most = ((int64_t)a.cols + 8191) / 8192;
+        int64_t parts = (512 + a.rows - 1) / a.rows;
+        if (parts > most) parts = most;
+        const dim3 grid((unsigned)(parts * a.rows));
+        if (a.cfg.top_k_rows || a.cfg.top_k > 0)
+            for (int level = 0; level < kUsedLevels<DT>; level++) {
+                GS_LAUNCH((k_long_digit<DT, OPACITY, false>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
+                GS_LAUNCH_CHECK();
+            }
+        if (a.cfg.top_p_rows || a.cfg.top_p < 1.0f)
+            for (int level = 0; level < kUsedLevels<DT>; level++) {
+                GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
+                GS_LAUNCH_CHECK();
+            }
+    }
+    if (begun) {
+        GS_LAUNCH((k_long_sums<DT, OPACITY, CUT, true>), chunks, dim3(kChunkThreads), 0, s, a, g);
+    } else {
+        GS_LAUNCH((k_long_sums<DT, OPACITY, false, false>), chunks, dim3(kChunkThreads), 0, s, a, g);
+    }
+    GS_LAUNCH_CHECK();
+    GS_LAUNCH((k_long_scan<DT, OPACITY, CUT>), rows, dim3(kHistThreads), 0, s, a, g);
+    GS_LAUNCH_CHECK();
+    const int64_t want = ((int64_t)a.rows * a.draws + 255) / 256;
+    GS_LAUNCH((k_long_draw<DT, OPACITY, CUT>), dim3((unsigned)want), dim3(256), 0, s, a, g, uniforms, ids);
+    GS_LAUNCH_CHECK();
+    return GS_OK;
+}
+
+template <int DT, bool OPACITY>
+static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *ids, char *ws, const SampleLayout &L,
+                         hipStream_t s) {
+    if (L.chunks == 0) return launch_rows<DT, OPACITY>(a, uniforms, ids, s);
+    const LongArgs g = {(LongRow *)(ws + L.rows), (uint64_t *)(ws + L.mass), (uint32_t *)(ws + L.count),
+                        (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
+                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint32_t *)(ws + L.seg_ties),
+                        L.chunks};
+    const GsSampleConfig &c = a.cfg;
+    const bool cut = c.top_k_rows || c.top_k > 0 || c.top_p_rows || c.top_p < 1.0f;
+    return cut ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
+               : launch_long<DT, OPACITY, false>(a, g, uniforms, ids, s);
 }
 
 }  // namespace gs
@@ -338,10 +946,15 @@ extern "C" int gs_sample(int rows, int cols, const void *logits, int64_t row_str
     const size_t size = cfg->dtype == kF32 ? 4 : 2;
     if (((uintptr_t)logits & (size - 1)) || ((uintptr_t)workspace & 15) || (((uintptr_t)uniforms | (uintptr_t)ids) & 3))
         return GS_ERR_INVALID_ARGUMENT;
-    if ((int64_t)rows * draws > 0x7fffffffLL * 128) return GS_ERR_INVALID_ARGUMENT;
     const SampleLayout L(rows, cols);
+    // a launch's workgroups, 31 bits
+    if (((int64_t)rows * draws + 255) / 256 > 0x7fffffffLL || (int64_t)rows * L.chunks > 0x7fffffffLL)
+        return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < L.total) return GS_ERR_WORKSPACE;
-    SampleArgs a = {logits, row_stride, rows, cols, draws, *cfg};
+    SampleArgs a = {logits, row_stride, rows, cols, draws, 0.0, *cfg};
+    int log_cols = 0;
+    while (((int64_t)1 << log_cols) < cols) log_cols++;
+    a.unit = ldexp(1.0, log_cols < 12 ? 50 : 62 - log_cols);
     const bool op = cfg->flags & GS_FLAG_LOGIT_OPACITY;
     hipStream_t s = (hipStream_t)stream;
     char *ws = (char *)workspace;

@@ -19,8 +19,7 @@ def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, opacity=Fal
         v = -np.logaddexp(np.longdouble(0), -v)
     with np.errstate(invalid="ignore"):
         d = np.where(v == v.max(), 0, v - v.max()) / np.longdouble(temperature if temperature > 0 else 1.0)
-    # (weights are 64-bit by definition: what lies below their range weighs nothing)
-    w = np.where(d < np.log(np.longdouble(2.0) ** -1074), 0, np.exp(d))
+    w = np.exp(d)
     order = np.argsort(-x[at], kind="stable")
     n = order.size
     if top_k > 0:
@@ -33,8 +32,11 @@ def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, opacity=Fal
     kept = np.sort(order[:n])
     if n > 1:
         kept = kept[w[kept] >= np.longdouble(np.float32(min_p))]
-    kept = kept[w[kept] > 0]
-    mass = np.cumsum(w[kept])
+    # (weights are rounded once, by definition)
+    unit = np.longdouble(2.0) ** min(50, 62 - int(np.ceil(np.log2(max(x.size, 2)))))
+    q = np.rint(w * unit)
+    kept = kept[q[kept] > 0]
+    mass = np.cumsum(q[kept])
     pick = np.searchsorted(mass, np.clip(np.nan_to_num(np.asarray(u, np.longdouble)), 0, 1) * mass[-1], side="right")
     return np.where(np.isnan(u), -1, at[kept[np.minimum(pick, kept.size - 1)]]).astype(np.int32)
 
