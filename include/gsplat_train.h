@@ -66,7 +66,7 @@ int gs_main_loss(int W, int H, const float *rendered, const float *gt, float ssi
  *   flags       GS_FLAG_LOGIT_OPACITY: v_opacity is the gradient w.r.t. the opacity logit (times o (1 - o));
  *               GS_FLAG_ACCUMULATE_GRADS: added to v_opacity (next to gs_gaussian_backward's) instead of written
  * Sums are 64-bit in a fixed order: equal calls give equal bits. */
-size_t gs_tile_balance_workspace_bytes(int W, int H);
+size_t gs_tile_balance_workspace_bytes(int W, int H, int N);
 int gs_tile_balance(int W, int H, int N, const float *packed, const int32_t *tile_bins, float scale, float *loss,
                     int32_t *counts, float *v_opacity, uint32_t flags, void *workspace, size_t workspace_bytes,
                     gs_stream_t stream);

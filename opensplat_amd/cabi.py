@@ -85,7 +85,7 @@ def lib() -> C.CDLL:
         l.gs_loss_workspace_bytes.argtypes = [C.c_int, C.c_int]
         l.gs_densify_workspace_bytes.restype = C.c_size_t
         l.gs_densify_workspace_bytes.argtypes = [C.c_int]
-        for fn, args in (("gs_tile_balance", [C.c_int] * 2), ("gs_sample", [C.c_int] * 2),
+        for fn, args in (("gs_tile_balance", [C.c_int] * 3), ("gs_sample", [C.c_int] * 2),
                          ("gs_relocate", [C.c_int] * 2)):
             getattr(l, fn + "_workspace_bytes").restype = C.c_size_t
             getattr(l, fn + "_workspace_bytes").argtypes = args
@@ -695,7 +695,7 @@ def tile_balance(W, H, packed, tile_bins, scale=1.0, flags=0, want_grad=True, ou
         if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev):
             raise ValueError("out must be (float32 [1], int32 [%d], float32 [%d]) on %s" % (tiles, N, dev))
     with torch.cuda.device(dev):
-        need = lib().gs_tile_balance_workspace_bytes(W, H)
+        need = lib().gs_tile_balance_workspace_bytes(W, H, N)
         if workspace is None or workspace.numel() < need:
             workspace = torch.empty(need, device=dev, dtype=torch.uint8)
         _check(lib().gs_tile_balance(W, H, N, _p(packed), _p(tile_bins), scale, _p(loss), _p(counts), _p(v), flags,

@@ -13,10 +13,14 @@
 //   k_relocate_claim   a target belongs to the first pair that names it; every target of a pair in range is marked
 //   k_relocate_count   pairs that hold (own target, source that is no target) are counted per source; the pair that is
 //                      counted first also rewrites the source — which one that is changes no result
-//   k_relocate_rows    64 pairs per workgroup: one lane each for opacity and extent, then their rows, a wave per pair
+//   k_relocate_rows    16 pairs per workgroup: one lane each for opacity and extent, then their rows, a wave for four pairs
+//                      with a lane per column of the six tensors, so that a row is one load and its copy one store
 // A source's opacity and scales are rewritten by one workgroup while others may hold pairs of the same source: those
 // columns are read by k_relocate_count, which writes no row, and kept per pair; k_relocate_rows reads only columns that
 // stay as they are.
+//
+// Bound by scattered lines: a row of 59 floats lies in six places (some nine 64-byte lines), written for the copy in
+// parameters and moments, and in the moments for the source.
 #include <math.h>
 
 #include "gs_device.h"
@@ -76,71 +80,94 @@ k_relocate_count(int N, int pairs, const int32_t *__restrict__ targets, const in
 
 struct RelocateSets {
     float *p[6], *m[6], *v[6];
-    int rest_len;
+    int columns;                               // floats per Gaussian over the six tensors
 };
 
-// log(o / D) and the new logit of a source with `m` equal shares
-static __device__ __forceinline__ void share(float logit, int m, double min_logit, float &new_logit, float &shrink) {
-    const double x = fmin((double)logit, 16.0);
-    const double big = (x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x)));   // softplus = -log(1 - o)
-    const double y = big / (double)m, p = -expm1(-y);
-    double term = 1.0, sum = 0.0;
+constexpr int kRowPairs = 16;
+
+// log(o / D) and the new logit of a source with `m` equal shares; `inverse` [j] = {1 / j, 1 / sqrt(j)}
+static __device__ __forceinline__ void share(float logit, int m, double min_logit, const double2 *inverse, float &new_logit,
+                                             float &shrink) {
+    const double x = fmin((double)logit, 16.0), z = log1p(exp(-fabs(x)));
+    const double y = (fmax(x, 0.0) + z) / (double)m, p = -expm1(-y);   // softplus / m = -log(1 - o) / m
+    double term = 1.0, sum = 0.0, left = (double)m * p;
     for (int j = 1; j <= kRelTerms && j <= m; j++) {
-        term *= (double)(m - j + 1) / (double)j * p;
-        const double t = term / sqrt((double)j);
-        sum += (j & 1) ? t : -t;
+        const double2 r = inverse[j];
+        term *= left * r.x;                    // C(m, j) p^j
+        left -= p;
+        sum += (j & 1) ? term * r.y : -(term * r.y);
         if (term < 1e-18 * sum) break;
     }
-    const double log_o = x < 0.0 ? x - log1p(exp(x)) : -log1p(exp(-x));
     new_logit = (float)fmax(log(expm1(y)), min_logit);
-    shrink = (float)(log_o - log(sum));
+    shrink = (float)(fmin(x, 0.0) - z - log(sum));
 }
 
 __global__ void __launch_bounds__(kRelThreads)
 k_relocate_rows(int pairs, const int32_t *__restrict__ targets, const int32_t *__restrict__ sources,
                 const int32_t *__restrict__ copies, const RelocatePair *__restrict__ in, double min_logit,
                 RelocateSets a) {
-    __shared__ float4 fresh[64];               // new logit, new log-scales
-    __shared__ int32_t rank[64];
-    const int tid = threadIdx.x, first = blockIdx.x * 64;
-    if (tid < 64) {
-        const int i = first + tid;
-        rank[tid] = -1;
-        if (i < pairs) {
-            const RelocatePair p = in[i];
-            rank[tid] = p.rank;
-            if (p.rank >= 0) {
-                float l, d;
-                share(p.logit, copies[sources[i]] + 1, min_logit, l, d);
-                fresh[tid] = make_float4(l, p.s0 + d, p.s1 + d, p.s2 + d);
-            }
+    __shared__ float fresh[kRowPairs][4];      // new log-scales, new logit
+    __shared__ int32_t rank[kRowPairs], to[kRowPairs], from[kRowPairs];
+    __shared__ double2 inverse[kRelTerms + 1];
+    const int tid = threadIdx.x, first = blockIdx.x * kRowPairs;
+    if (tid >= 64 && tid <= 64 + kRelTerms) {
+        const double j = tid > 64 ? (double)(tid - 64) : 1.0;
+        inverse[tid - 64] = make_double2(1.0 / j, 1.0 / sqrt(j));
+    }
+    RelocatePair p = {0.0f, 0.0f, 0.0f, 0.0f, -1};
+    int32_t s = 0, m = 0;
+    if (tid < kRowPairs && first + tid < pairs) {
+        p = in[first + tid];
+        if (p.rank >= 0) {
+            s = sources[first + tid];
+            m = copies[s] + 1;
+            to[tid] = targets[first + tid];
+            from[tid] = s;
         }
     }
     __syncthreads();
-    const int lane = tid & 63;
-    for (int k = tid >> 6; k < 64; k += kRelThreads / 64) {
-        const int rk = rank[k];
-        if (rk < 0) continue;
-        const size_t t = (size_t)targets[first + k], s = (size_t)sources[first + k];
-        const float4 f = fresh[k];
-        const int lens[6] = {3, 3, 4, 1, 3, a.rest_len};
-        for (int q = 0; q < 6; q++) {
-            const int len = lens[q];
-            for (int c = lane; c < len; c += 64) {
-                float v;
-                if (q == 1) v = c == 0 ? f.y : (c == 1 ? f.z : f.w);
-                else if (q == 3) v = f.x;
-                else v = a.p[q][s * len + c];
-                a.p[q][t * len + c] = v;
-                if (rk == 0 && (q == 1 || q == 3)) a.p[q][s * len + c] = v;
-                if (a.m[q]) {
-                    a.m[q][t * len + c] = 0.0f;
-                    if (rk == 0) a.m[q][s * len + c] = 0.0f;
-                }
-                if (a.v[q]) {
-                    a.v[q][t * len + c] = 0.0f;
-                    if (rk == 0) a.v[q][s * len + c] = 0.0f;
-                }
+    if (tid < kRowPairs) {
+        rank[tid] = p.rank;
+        if (p.rank >= 0) {
+            float l, d;
+            share(p.logit, m, min_logit, inverse, l, d);
+            fresh[tid][0] = p.s0 + d;
+            fresh[tid][1] = p.s1 + d;
+            fresh[tid][2] = p.s2 + d;
+            fresh[tid][3] = l;
+        }
+    }
+    __syncthreads();
+    const int lane = tid & 63, k0 = (tid >> 6) * (kRowPairs / 4);
+    for (int c0 = 0; c0 < a.columns; c0 += 64) {
+        const int c = c0 + lane;
+        if (c >= a.columns) continue;
+        // the lane's tensor, its row length and the column in it
+        float *tp = a.p[5], *tm = a.m[5], *tv = a.v[5];
+        int len = a.columns - 14, off = c - 14, q = -1;   // q: the column of `fresh`
+        if (c < 3) { tp = a.p[0]; tm = a.m[0]; tv = a.v[0]; len = 3; off = c; }
+        else if (c < 6) { tp = a.p[1]; tm = a.m[1]; tv = a.v[1]; len = 3; off = q = c - 3; }
+        else if (c < 10) { tp = a.p[2]; tm = a.m[2]; tv = a.v[2]; len = 4; off = c - 6; }
+        else if (c < 11) { tp = a.p[3]; tm = a.m[3]; tv = a.v[3]; len = 1; off = 0; q = 3; }
+        else if (c < 14) { tp = a.p[4]; tm = a.m[4]; tv = a.v[4]; len = 3; off = c - 11; }
+        float v[kRowPairs / 4];
+#pragma unroll
+        for (int k = 0; k < kRowPairs / 4; k++) {
+            v[k] = 0.0f;
+            if (rank[k0 + k] >= 0) v[k] = q >= 0 ? fresh[k0 + k][q] : tp[(size_t)from[k0 + k] * len + off];
+        }
+#pragma unroll
+        for (int k = 0; k < kRowPairs / 4; k++) {
+            const int32_t rk = rank[k0 + k];
+            if (rk < 0) continue;
+            const size_t t = (size_t)to[k0 + k] * len + off, f = (size_t)from[k0 + k] * len + off;
+            tp[t] = v[k];
+            if (tm) tm[t] = 0.0f;
+            if (tv) tv[t] = 0.0f;
+            if (rk == 0) {
+                if (q >= 0) tp[f] = v[k];
+                if (tm) tm[f] = 0.0f;
+                if (tv) tv[f] = 0.0f;
             }
         }
     }
@@ -194,9 +221,9 @@ extern "C" int gs_relocate(int N, int K, int pairs, const int32_t *targets, cons
     RelocateSets a = {{p.means, p.log_scales, p.quats, p.opacity_logits, p.features_dc, p.features_rest},
                       {m.means, m.log_scales, m.quats, m.opacity_logits, m.features_dc, m.features_rest},
                       {v.means, v.log_scales, v.quats, v.opacity_logits, v.features_dc, v.features_rest},
-                      (K - 1) * 3};
+                      14 + (K - 1) * 3};
     const double o = (double)min_opacity;
-    GS_LAUNCH(k_relocate_rows, dim3((pairs + 63) / 64), block, 0, s, pairs, targets, sources, copies, held,
+    GS_LAUNCH(k_relocate_rows, dim3((pairs + kRowPairs - 1) / kRowPairs), block, 0, s, pairs, targets, sources, copies, held,
               log(o / (1.0 - o)), a);
     GS_LAUNCH_CHECK();
     return GS_OK;

@@ -20,8 +20,7 @@
 //
 // Two forms, by the length of a row:
 //   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row)
-//   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*), the last
-//   workgroup of a row to finish a histogram picking the digit
+//   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*)
 #include <math.h>
 
 #include "gs_device.h"
@@ -118,10 +117,13 @@ static __device__ __forceinline__ void keys_at(const char *row, int64_t i, int64
 }
 
 // ---- weights ----------------------------------------------------------------------------------------------------
-// 2^y for y <= 0 by 2^n times the Taylor polynomial of 2^f, |f| <= 1/2: (ln 2 / 2)^13 / 13! = 2e-16.
+// 2^y for y <= 0 by 2^n times the Taylor polynomial of 2^f, |f| <= 1/2: (ln 2 / 2)^13 / 13! = 2e-16.  Adding 1.5 2^52
+// rounds y to the integer n and leaves n in the low word; it goes into the exponent by an integer addition (the slower
+// rint, ldexp and conversions cost as much as the polynomial).  Below 2^-1000: 2^-1000.
 static __device__ __forceinline__ double pow2(double y) {
-    y = fmax(y, -1100.0);
-    const double n = rint(y), f = y - n;
+    y = fmax(y, -1000.0);
+    const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+    const int n = (int)(uint32_t)__double_as_longlong(shifted);
     constexpr double L = 0.69314718055994530941723212145818;
     constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
                      c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11,
@@ -138,7 +140,7 @@ static __device__ __forceinline__ double pow2(double y) {
     p = fma(p, f, c2);
     p = fma(p, f, c1);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
 }
 constexpr double kLog2e = 1.4426950408889634073599246810019;
 
@@ -215,7 +217,7 @@ static __device__ __forceinline__ bool agrees(uint32_t key, uint32_t found, int 
     return level == 0 || (key >> (level == 1 ? 21 : 10)) == (found >> (level == 1 ? 21 : 10));
 }
 
-// One search, for top-k (counts) or top-p (masses), as it stands between two digits.
+// A search, for top-k (counts) or top-p (masses), as it stands between two digits.
 struct Search {
     uint64_t above;                            // count or mass over the digits found
     double goal;                               // count or mass to reach
@@ -457,31 +459,38 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
 }
 
 // ---- longer rows ------------------------------------------------------------------------------------------------------
-constexpr int kSeg = 16;                       // entries one thread sums: the grain of the stored running sums
+constexpr int kSeg = 8;                        // entries between two stored running sums
 constexpr int kChunkThreads = 256;
-constexpr int kChunk = kChunkThreads * kSeg;
+constexpr int kChunk = kChunkThreads * 2 * kSeg;
+constexpr int kChunkSegs = kChunk / kSeg;
+constexpr int kLevels = 3;
 constexpr int kHistThreads = 1024;
+constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
+constexpr int kCopies = 4;
 
-// A row's state between the launches.
+// A row's state between the launches.  A launch reads what earlier ones wrote and writes other fields.
 struct LongRow {
     double inv_t, top_p, min_p;
+    Scale scale;
     uint64_t total, tie_weight;
-    Search k, p;
-    uint32_t max_key, thr, ties, arrived;
+    Search k[kLevels], p[kLevels];             // as the launch of that digit found it
+    uint32_t k_thr, k_ties, thr, ties;
     int32_t top_k;
-    uint32_t ok, greedy, pad;
+    uint32_t ok, greedy;
 };
 
 struct LongArgs {
     LongRow *rows;
-    uint64_t *mass;                            // [rows][kBins]
-    uint32_t *count;                           // [rows][kBins]
+    uint32_t *k_count;                         // [rows][kLevels][kBins]
+    uint64_t *p_mass;                          // [rows][kLevels][kBins]
+    uint32_t *p_count;                         // [rows][kBins], of the last digit
     uint32_t *chunk_max;                       // [rows][chunks]
     uint64_t *chunk_sum;                       // [rows][chunks]: sums, then running sums
     uint32_t *chunk_ties;                      // [rows][chunks]: ties, then running ties
-    uint64_t *seg_sum;                           // [rows][chunks][256] running sums inside the chunk
-    uint32_t *seg_ties;                        // [rows][chunks][256]
+    uint64_t *seg_sum;                         // [rows][chunks][kChunkSegs] running sums inside the chunk
+    uint32_t *seg_ties;
     int chunks;
+    bool with_k, with_p;                       // launches that look for a threshold
 };
 
 template <int DT>
@@ -497,7 +506,7 @@ k_long_max(SampleArgs a, LongArgs g) {
     const char *row = row_base<DT>(a, r);
     uint32_t mx = 0;
 #pragma unroll
-    for (int q = 0; q < kSeg / kVec<DT>; q++) {
+    for (int q = 0; q < 2 * kSeg / kVec<DT>; q++) {
         uint32_t k[kVec<DT>];
         keys_at<DT>(row, (int64_t)c * kChunk + ((int64_t)q * kChunkThreads + tid) * kVec<DT>, a.cols, k);
 #pragma unroll
@@ -510,6 +519,7 @@ k_long_max(SampleArgs a, LongArgs g) {
 }
 
 // The row's settings and maximum, nothing cut yet.
+template <int DT, bool OPACITY>
 static __device__ __forceinline__ LongRow long_row(const SampleArgs &a, int r, uint32_t max_key) {
     const RowSettings set = row_settings(a, r);
     LongRow s = {};
@@ -519,10 +529,10 @@ static __device__ __forceinline__ LongRow long_row(const SampleArgs &a, int r, u
     s.top_k = set.top_k;
     s.ok = set.ok && max_key != 0;
     s.greedy = set.greedy;
-    s.max_key = max_key;
-    s.k.goal = (double)set.top_k;
-    s.k.done = set.greedy || !s.ok || set.top_k == 0;
-    s.p.done = set.greedy || !s.ok || !(set.top_p < 1.0);
+    s.scale = scale_for<DT, OPACITY>(max_key, set.inv_t);
+    s.k[0].goal = (double)set.top_k;
+    s.k[0].done = set.greedy || !s.ok || set.top_k == 0;
+    s.p[0].done = set.greedy || !s.ok || !(set.top_p < 1.0);
     return s;
 }
 
@@ -541,195 +551,313 @@ static __device__ __forceinline__ uint32_t row_max(const LongArgs &g, int r, uin
 }
 
 // One workgroup per row: its state, empty histograms.
+template <int DT, bool OPACITY>
 __global__ void __launch_bounds__(kHistThreads)
-k_long_begin(SampleArgs a, LongArgs g, int histograms) {
+k_long_begin(SampleArgs a, LongArgs g) {
     __shared__ uint32_t waves[kHistThreads / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
-    if (histograms)
-        for (int b = tid; b < kBins; b += kHistThreads) {
-            g.mass[(size_t)r * kBins + b] = 0;
-            g.count[(size_t)r * kBins + b] = 0;
-        }
+    constexpr int used = kUsedLevels<DT> * kBins;
+    for (int b = tid; b < used; b += kHistThreads) {
+        if (g.with_k) g.k_count[(size_t)r * kLevels * kBins + b] = 0;
+        if (g.with_p) g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
+    }
+    if (g.with_p)
+        for (int b = tid; b < kBins; b += kHistThreads) g.p_count[(size_t)r * kBins + b] = 0;
     const uint32_t mx = row_max<kHistThreads>(g, r, waves);
-    if (tid == 0) g.rows[r] = long_row(a, r, mx);
+    if (tid == 0) g.rows[r] = long_row<DT, OPACITY>(a, r, mx);
 }
 
-// A digit of the top-k threshold (MASS false) or of the top-p threshold.  `parts` workgroups per row; each adds its
-// part's histogram to the row's, and the last of them to arrive picks the digit and empties the row's histogram again.
-// The row's counters are only touched by device-wide atomics here: the caches of the eight dies do not see each other's
-// plain stores within a launch.
+// The state behind digit `level`, from its histogram; by every workgroup for itself, so that no launch waits for a last
+// one.  `count` gets how many entries have that digit (top-p, last digit).
+template <int DT>
+static __device__ __forceinline__ Search after_k(const LongArgs &g, int r, int level, const Search &f, uint64_t *waves_u,
+                                                 Picked *pick) {
+    if (f.done) return f;
+    const uint32_t *bins = g.k_count + ((size_t)r * kLevels + level) * kBins;
+    const Picked p = pick_digit<kHistThreads>([&](int i) { return (uint64_t)bins[i]; }, f.above, f.goal, false, 0.0,
+                                              waves_u, pick);
+    Search next = f;
+    if (p.digit == kBins) next.done = 1;       // fewer candidates than k
+    else next.found |= p.digit << digit_shift(level);
+    next.above = p.above;
+    return next;
+}
+template <int DT, bool OPACITY>
+static __device__ __forceinline__ Search after_p(const SampleArgs &a, const LongArgs &g, int r, int level, const Search &f,
+                                                 const LongRow &st, uint32_t k_thr, uint32_t k_ties, uint64_t *waves_u,
+                                                 Picked *pick, uint64_t *have) {
+    if (f.done) return f;
+    // the ties that top-k left count as one entry of k_ties times the weight
+    uint64_t tied = 0;
+    int tied_digit = -1;
+    if (k_thr && agrees(k_thr, f.found, level)) {
+        tied = (uint64_t)k_ties * fixed(weight<DT, OPACITY>(k_thr, st.scale), a.unit);
+        tied_digit = (int)digit_of(k_thr, level);
+    }
+    const uint64_t *bins = g.p_mass + ((size_t)r * kLevels + level) * kBins;
+    const Picked p = pick_digit<kHistThreads>([&](int i) { return bins[i] + (i == tied_digit ? tied : 0ull); }, f.above,
+                                              f.goal, level == 0, st.top_p, waves_u, pick);
+    Search next = f;
+    if (level == 0) next.goal = st.top_p * (double)p.total;
+    if (p.digit == kBins) {
+        next.done = 1;
+    } else {
+        next.found |= p.digit << digit_shift(level);
+        next.above = p.above;
+        *have = (uint64_t)g.p_count[(size_t)r * kBins + p.digit] + ((int)p.digit == tied_digit ? k_ties : 0u);
+    }
+    return next;
+}
+// The top-k threshold, once all its digits are counted.
+template <int DT>
+static __device__ __forceinline__ void finish_k(const LongArgs &g, int r, const LongRow &st, uint64_t *waves_u,
+                                                Picked *pick, uint32_t &thr, uint32_t &ties) {
+    constexpr int last = kUsedLevels<DT> - 1;
+    thr = ties = 0;
+    if (!g.with_k) return;
+    const Search f = after_k<DT>(g, r, last, st.k[last], waves_u, pick);
+    if (f.done) return;
+    thr = f.found;
+    ties = (uint32_t)st.top_k - (uint32_t)f.above;
+}
+
+// The histogram of a digit of the top-k threshold (MASS false) or of the top-p threshold; `parts` workgroups per row.
+// Bound by the loads' latency and by fp64: some 40 instructions a weight, 75 for an opacity's power.
 template <int DT, bool OPACITY, bool MASS>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
-    __shared__ uint64_t mass[MASS ? kBins : 1];
+    // Neighbouring values share a first digit, a wave's atomics then hit few words: four copies of the masses, by lane.
+    __shared__ uint64_t mass[MASS ? kBins * kCopies : 1];
     __shared__ uint32_t count[kBins];
     __shared__ uint64_t waves_u[kHistThreads / 64];
     __shared__ Picked pick;
-    __shared__ uint32_t last;
     const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
     LongRow &st = g.rows[r];
-    const Search f = MASS ? st.p : st.k;
+    uint32_t k_thr = 0, k_ties = 0;
+    Search f;
+    if constexpr (MASS) {
+        if (level == 0) {
+            f = st.p[0];
+            if (!f.done) {
+                finish_k<DT>(g, r, st, waves_u, &pick, k_thr, k_ties);
+                if (part == 0 && tid == 0) {
+                    st.k_thr = k_thr;
+                    st.k_ties = k_ties;
+                }
+            }
+        } else {
+            k_thr = st.k_thr;
+            k_ties = st.k_ties;
+            uint64_t have;
+            f = after_p<DT, OPACITY>(a, g, r, level - 1, st.p[level - 1], st, k_thr, k_ties, waves_u, &pick, &have);
+        }
+    } else {
+        f = level == 0 ? st.k[0] : after_k<DT>(g, r, level - 1, st.k[level - 1], waves_u, &pick);
+    }
+    if (level > 0 && part == 0 && tid == 0) (MASS ? st.p : st.k)[level] = f;
     if (f.done) return;
     const bool final_level = level == kUsedLevels<DT> - 1;
-    const uint32_t kthr = MASS ? st.thr : 0u, kties = MASS ? st.ties : 0u;
-    const Scale s = scale_for<DT, OPACITY>(st.max_key, st.inv_t);
+    const Scale s = st.scale;
+    // Where few entries agree, a wave would compute a weight for a lane or two of every 64: they are queued (in the space
+    // of the copies, which such a histogram does without), and taken 64 at a time.
+    const bool queued = MASS && (level > 0 || k_thr != 0);
+    const int copies = (MASS && !queued) ? kCopies : 1;
     for (int b = tid; b < kBins; b += kHistThreads) {
-        if constexpr (MASS) mass[b] = 0;
+        if constexpr (MASS)
+            for (int c = 0; c < copies; c++) mass[b * copies + c] = 0;
         count[b] = 0;
     }
     __syncthreads();
     const char *row = row_base<DT>(a, r);
-    const int64_t n = a.cols;
-    for (int64_t i = ((int64_t)part * kHistThreads + tid) * kVec<DT>; i < n; i += (int64_t)parts * kHistThreads * kVec<DT>) {
-        uint32_t k[kVec<DT>];
-        keys_at<DT>(row, i, n, k);
-#pragma unroll
-        for (int e = 0; e < kVec<DT>; e++) {
-            if (!(k[e] > kthr) || !agrees(k[e], f.found, level)) continue;
-            const uint32_t d = digit_of(k[e], level);
-            if constexpr (MASS) {
-                atomicAdd((unsigned long long *)&mass[d],
-                          (unsigned long long)fixed(weight<DT, OPACITY>(k[e], s), a.unit));
-                if (final_level) atomicAdd(&count[d], 1u);
-            } else {
-                atomicAdd(&count[d], 1u);
-            }
+    const int64_t n = a.cols, step = (int64_t)kHistThreads * kVec<DT>;
+    const int lane = tid & 63, copy = lane & (copies - 1);
+    auto add = [&](uint32_t key) {
+        const uint32_t d = digit_of(key, level);
+        if constexpr (MASS) {
+            atomicAdd((unsigned long long *)&mass[d * copies + copy],
+                      (unsigned long long)fixed(weight<DT, OPACITY>(key, s), a.unit));
+            if (final_level) atomicAdd(&count[d], 1u);
+        } else {
+            atomicAdd(&count[d], 1u);
         }
+    };
+    uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? kBins : 0)) + (tid >> 6) * 128;
+    int waiting = 0;
+    for (int64_t i0 = (int64_t)part * kBatch * step + (int64_t)tid * kVec<DT>; i0 - (int64_t)tid * kVec<DT> < n;
+         i0 += (int64_t)parts * kBatch * step) {
+        uint32_t k[kBatch][kVec<DT>];
+#pragma unroll
+        for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + q * step, n, k[q]);
+#pragma unroll
+        for (int q = 0; q < kBatch; q++)
+#pragma unroll
+            for (int e = 0; e < kVec<DT>; e++) {
+                const bool in = k[q][e] > k_thr && agrees(k[q][e], f.found, level);
+                if (!queued) {
+                    if (in) add(k[q][e]);
+                    continue;
+                }
+                const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+                if (m == 0) continue;
+                if (in) wave_queue[waiting + __builtin_popcountll(m & ((1ull << lane) - 1ull))] = k[q][e];
+                waiting += __builtin_popcountll(m);
+                if (waiting >= 64) {
+                    waiting -= 64;
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    add(wave_queue[waiting + lane]);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
+            }
+    }
+    if (queued) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lane < waiting) add(wave_queue[lane]);
     }
     __syncthreads();
-    uint64_t *row_mass = g.mass + (size_t)r * kBins;
-    uint32_t *row_count = g.count + (size_t)r * kBins;
-    for (int b = tid; b < kBins; b += kHistThreads) {
-        if constexpr (MASS)
-            if (mass[b]) atomicAdd((unsigned long long *)&row_mass[b], (unsigned long long)mass[b]);
-        if (count[b]) atomicAdd(&row_count[b], count[b]);
-    }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) last = __hip_atomic_fetch_add(&st.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
     for (int b = tid; b < kBins; b += kHistThreads) {
         if constexpr (MASS) {
-            mass[b] = __hip_atomic_load(&row_mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&row_mass[b], (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        count[b] = __hip_atomic_load(&row_count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&row_count[b], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (MASS && tid == 0 && kthr && agrees(kthr, f.found, level)) {   // the ties that top-k left, as one
-        const uint32_t d = digit_of(kthr, level);
-        mass[MASS ? d : 0] += (uint64_t)kties * fixed(weight<DT, OPACITY>(kthr, s), a.unit);
-        count[d] += kties;
-    }
-    __syncthreads();
-    const Picked p = pick_digit<kHistThreads>([&](int i) { return MASS ? mass[MASS ? i : 0] : (uint64_t)count[i]; }, f.above,
-                                              f.goal, MASS && level == 0, st.top_p, waves_u, &pick);
-    if (tid == 0) {
-        Search next = f;
-        if (MASS && level == 0) next.goal = st.top_p * (double)p.total;
-        if (p.digit == kBins) {
-            next.done = 1;
+            uint64_t m = 0;
+            for (int c = 0; c < copies; c++) m += mass[b * copies + c];
+            if (m) atomicAdd((unsigned long long *)&g.p_mass[((size_t)r * kLevels + level) * kBins + b], (unsigned long long)m);
+            if (final_level && count[b]) atomicAdd(&g.p_count[(size_t)r * kBins + b], count[b]);
         } else {
-            next.found |= p.digit << digit_shift(level);
-            next.above = p.above;
-            if (final_level) {
-                st.thr = next.found;
-                st.ties = MASS ? ties_for(next.above, next.goal, weight<DT, OPACITY>(next.found, s), a.unit, count[p.digit])
-                               : (uint32_t)st.top_k - (uint32_t)next.above;
-            }
+            if (count[b]) atomicAdd(&g.k_count[((size_t)r * kLevels + level) * kBins + b], count[b]);
         }
-        if (MASS) st.p = next;
-        else st.k = next;
-        st.arrived = 0;
     }
 }
 
-// Per chunk: running sums of the kept weights and of the ties per 16 entries, and their totals.  CUT false: no row has a
+// One workgroup per row: threshold and ties, once all digits are counted.
+template <int DT, bool OPACITY>
+__global__ void __launch_bounds__(kHistThreads)
+k_long_cut(SampleArgs a, LongArgs g) {
+    __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ Picked pick;
+    const int r = blockIdx.x;
+    LongRow &st = g.rows[r];
+    constexpr int last = kUsedLevels<DT> - 1;
+    uint32_t thr = 0, ties = 0;
+    if (g.with_p && !st.p[0].done) {
+        thr = st.k_thr;
+        ties = st.k_ties;
+        uint64_t have = 0;
+        const Search f = after_p<DT, OPACITY>(a, g, r, last, st.p[last], st, thr, ties, waves_u, &pick, &have);
+        if (!f.done) {
+            thr = f.found;
+            ties = ties_for(f.above, f.goal, weight<DT, OPACITY>(thr, st.scale), a.unit, have);
+        }
+    } else {
+        finish_k<DT>(g, r, st, waves_u, &pick, thr, ties);
+    }
+    if (threadIdx.x == 0) {
+        st.thr = thr;
+        st.ties = ties;
+        st.tie_weight = 0;
+        if (thr) {
+            const double w = weight<DT, OPACITY>(thr, st.scale);
+            st.tie_weight = w >= st.min_p ? fixed(w, a.unit) : 0ull;
+        }
+    }
+}
+
+// Per chunk: running sums of the kept weights and of the ties per 8 entries, and their totals.  CUT false: no row has a
 // threshold, and (BEGUN false) no launch has prepared the rows' state: the row's maximum is taken from its chunks' here.
 template <int DT, bool OPACITY, bool CUT, bool BEGUN>
 __global__ void __launch_bounds__(kChunkThreads)
 k_long_sums(SampleArgs a, LongArgs g) {
     __shared__ uint64_t waves_u[kChunkThreads / 64];
     __shared__ uint32_t waves_i[kChunkThreads / 64];
+    __shared__ uint32_t keys[CUT ? 2 * kSeg : 1][kChunkThreads];
     const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
     const char *row = row_base<DT>(a, r);
-    const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * kSeg;
-    uint32_t key[kSeg];
+    const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * 2 * kSeg;
+    uint32_t key[2 * kSeg];
 #pragma unroll
-    for (int q = 0; q < kSeg / kVec<DT>; q++) {
+    for (int q = 0; q < 2 * kSeg / kVec<DT>; q++) {
         uint32_t k[kVec<DT>];
         keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
 #pragma unroll
         for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
     }
-    uint32_t top, thr = 0;
-    double inv_t, min_p;
+    uint32_t thr = 0;
+    double min_p;
+    Scale s;
     bool greedy, ok;
+    uint64_t tie_weight = 0;
     if constexpr (BEGUN) {
         const LongRow &st = g.rows[r];
-        top = st.max_key;
         thr = CUT ? st.thr : 0u;
-        inv_t = st.inv_t;
+        tie_weight = CUT ? st.tie_weight : 0ull;
+        s = st.scale;
         min_p = st.min_p;
         greedy = st.greedy;
         ok = st.ok;
     } else {
-        top = row_max<kChunkThreads>(g, r, waves_i);
-        const LongRow st = long_row(a, r, top);
-        inv_t = st.inv_t;
+        const LongRow st = long_row<DT, OPACITY>(a, r, row_max<kChunkThreads>(g, r, waves_i));
+        s = st.scale;
         min_p = st.min_p;
         greedy = st.greedy;
         ok = st.ok;
         if (c == 0 && tid == 0) g.rows[r] = st;
     }
-    const Scale s = scale_for<DT, OPACITY>(top, inv_t);
-    uint64_t sum = 0;
-    uint32_t ties = 0;
+    uint64_t sum[2] = {0, 0};
+    uint32_t ties[2] = {0, 0};
     if (ok) {
+        uint32_t above = 0;
 #pragma unroll
-        for (int e = 0; e < kSeg; e++) {
-            if (CUT && thr) ties += key[e] == thr;
-            if (!(key[e] > thr) || (greedy && key[e] != top)) continue;
-            const double w = weight<DT, OPACITY>(key[e], s);
-            if (w >= min_p) sum += fixed(w, a.unit);
+        for (int e = 0; e < 2 * kSeg; e++) {
+            if (CUT && thr) ties[e / kSeg] += key[e] == thr;
+            above |= (key[e] > thr && (!greedy || key[e] == s.top)) ? 1u << e : 0u;
+        }
+        if constexpr (CUT) {
+            // A lane goes through its own kept entries: behind a cut a wave takes as many rounds as its fullest lane has,
+            // not sixteen with a few lanes each.
+#pragma unroll
+            for (int e = 0; e < 2 * kSeg; e++) keys[e][tid] = key[e];
+            while (above) {
+                const int e = __builtin_ctz(above);
+                above &= above - 1;
+                const double w = weight<DT, OPACITY>(keys[e][tid], s);
+                if (w >= min_p) sum[e >= kSeg ? 1 : 0] += fixed(w, a.unit);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2 * kSeg; e++) {
+                const double w = weight<DT, OPACITY>(key[e], s);
+                if (((above >> e) & 1u) && w >= min_p) sum[e / kSeg] += fixed(w, a.unit);
+            }
         }
     }
-    const size_t at = (size_t)r * g.chunks + c;
-    const size_t seg = at * kChunkThreads + tid;
+    if constexpr (CUT) {                       // (as if all ties were kept: see ChunkView)
+        sum[0] += tie_weight * ties[0];
+        sum[1] += tie_weight * ties[1];
+    }
+    const size_t at = (size_t)r * g.chunks + c, seg = at * kChunkSegs + 2 * tid;
     uint64_t total;
-    g.seg_sum[seg] = block_scan<kChunkThreads>(sum, waves_u, total);
+    const uint64_t before = block_scan<kChunkThreads>(sum[0] + sum[1], waves_u, total);
+    *reinterpret_cast<ulonglong2 *>(g.seg_sum + seg) = make_ulonglong2(before, before + sum[0]);
     if (tid == 0) g.chunk_sum[at] = total;
     if constexpr (CUT) {
-        uint32_t all = 0, ties_before = 0;
-        if (thr) ties_before = block_scan<kChunkThreads>(ties, waves_i, all);
-        g.seg_ties[seg] = ties_before;
-        if (tid == 0) g.chunk_ties[at] = all;
+        if (thr) {
+            uint32_t all;
+            const uint32_t ties_before = block_scan<kChunkThreads>(ties[0] + ties[1], waves_i, all);
+            *reinterpret_cast<uint2 *>(g.seg_ties + seg) = make_uint2(ties_before, ties_before + ties[0]);
+            if (tid == 0) g.chunk_ties[at] = all;
+        }
     }
 }
 
 // One workgroup per row: running sums over the chunks.
-template <int DT, bool OPACITY, bool CUT>
+template <bool CUT>
 __global__ void __launch_bounds__(kHistThreads)
-k_long_scan(SampleArgs a, LongArgs g) {
+k_long_scan(LongArgs g) {
     __shared__ uint64_t waves_u[kHistThreads / 64];
     __shared__ uint32_t waves_i[kHistThreads / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
     LongRow &st = g.rows[r];
     const size_t first = (size_t)r * g.chunks;
     const bool ok = st.ok;
-    uint32_t thr = 0, ties = 0;
-    uint64_t tie_weight = 0;
-    if constexpr (CUT) {
-        thr = st.thr;
-        ties = st.ties;
-        if (thr) {
-            const double w = weight<DT, OPACITY>(thr, scale_for<DT, OPACITY>(st.max_key, st.inv_t));
-            tie_weight = w >= st.min_p ? fixed(w, a.unit) : 0ull;
-        }
-    }
+    const uint32_t thr = CUT ? st.thr : 0u, ties = CUT ? st.ties : 0u;
+    const uint64_t tie_weight = CUT ? st.tie_weight : 0ull;
     uint64_t base = 0;
     uint32_t tie_base = 0;
     for (int c0 = 0; c0 < g.chunks; c0 += kHistThreads) {
@@ -742,28 +870,101 @@ k_long_scan(SampleArgs a, LongArgs g) {
             const uint32_t before = tie_base + block_scan<kHistThreads>(here, waves_i, all);
             tie_base += all;
             if (in) g.chunk_ties[first + c] = before;
-            v += tie_weight * min(ties > before ? ties - before : 0u, here);
+            const uint32_t left = ties > before ? ties - before : 0u;
+            if (left < here) v -= tie_weight * (here - left);
         }
         uint64_t all;
         const uint64_t before = base + block_scan<kHistThreads>(v, waves_u, all);
         base += all;
         if (in) g.chunk_sum[first + c] = before;
     }
-    if (tid == 0) {
-        st.total = ok ? base : 0ull;
-        st.tie_weight = tie_weight;
-    }
+    if (tid == 0) st.total = ok ? base : 0ull;
 }
 
-// One thread per draw: the last chunk, then the last 16 entries, whose running sum does not exceed the goal, then entry by
-// entry.  (Integer sums: what is found there holds a weight.)
+// The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not exceed `goal`; four-fold steps, whose three
+// loads are under way together.
+template <typename F>
+static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f) {
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 3) >> 2;
+        uint64_t v[3];
+#pragma unroll
+        for (int j = 0; j < 3; j++) v[j] = (j + 1) * step < n ? f(lo + (j + 1) * step) : ~0ull;
+        const int c = (v[0] <= goal) + (v[1] <= goal) + (v[2] <= goal);
+        lo += c * step;
+        n = min(step, n - c * step);
+    }
+    return lo;
+}
+// The same by a wave, 64 values at a time; every lane gets it.
+template <typename F>
+static __device__ __forceinline__ int wave_last_not_above(int n, uint64_t goal, F f) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const bool below = at < n && f(lo + at) <= goal;
+        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(below)) - 1;   // (f(lo) <= goal)
+        lo += c * step;
+        n = min(step, n - c * step);
+    }
+    return lo;
+}
+
+// A chunk's running sums as the draws see them.  The stored ones hold all of the chunk's ties; where not all are kept, the
+// ones behind the `left` first are taken off.
+template <bool CUT>
+struct ChunkView {
+    const uint64_t *seg_sum;
+    const uint32_t *seg_ties;
+    uint64_t tie_weight;
+    uint32_t thr, left;
+    bool cut;
+    __device__ ChunkView(const LongArgs &g, const LongRow &st, int r, int c) {
+        const size_t chunk = (size_t)r * g.chunks + c;
+        seg_sum = g.seg_sum + chunk * kChunkSegs;
+        seg_ties = g.seg_ties + chunk * kChunkSegs;
+        tie_weight = 0;
+        thr = CUT ? st.thr : 0u;
+        left = 0xffffffffu;
+        cut = false;
+        if (CUT && thr) {
+            tie_weight = st.tie_weight;
+            const uint32_t before = g.chunk_ties[chunk];
+            left = st.ties > before ? st.ties - before : 0u;
+            cut = c + 1 == g.chunks || g.chunk_ties[chunk + 1] - before > left;
+        }
+    }
+    __device__ uint64_t sum_before(int i) const {
+        uint64_t v = seg_sum[i];
+        if (CUT && cut) {
+            const uint32_t t = seg_ties[i];
+            if (t > left) v -= tie_weight * (t - left);
+        }
+        return v;
+    }
+};
+
+// Many draws: one thread each.  The last chunk, then the last 8 entries, whose running sum does not exceed the goal, then
+// entry by entry.  (Integer sums: what is found there holds a weight.)  A workgroup's draws are of one row; its chunks'
+// running sums are searched in LDS where they fit.
+constexpr int kDrawThreads = 256;
+constexpr int kDrawChunks = 4096;
 template <int DT, bool OPACITY, bool CUT>
-__global__ void __launch_bounds__(256)
-k_long_draw(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (at >= (int64_t)a.rows * a.draws) return;
-    const int r = (int)(at / a.draws);
+__global__ void __launch_bounds__(kDrawThreads)
+k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+    extern __shared__ uint64_t sums[];
+    const int r = blockIdx.x / blocks, j = (blockIdx.x - r * blocks) * kDrawThreads + threadIdx.x;
     const LongRow &st = g.rows[r];
+    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
+    const bool staged = g.chunks <= kDrawChunks;
+    if (staged) {
+        for (int c = threadIdx.x; c < g.chunks; c += kDrawThreads) sums[c] = chunk_sum[c];
+        __syncthreads();
+    }
+    if (j >= a.draws) return;
+    const size_t at = (size_t)r * a.draws + j;
     const uint64_t total = st.total;
     const float u = uniforms[at];
     if (total == 0 || isnan(u)) {
@@ -772,68 +973,92 @@ k_long_draw(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_
     }
     const bool greedy = st.greedy;
     const uint64_t goal = greedy ? 0ull : goal_of(u, total);
-    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-    int lo = 0, hi = g.chunks;                 // chunk_sum[lo] <= goal < chunk_sum[hi]
-    while (hi - lo > 1) {
-        const int mid = lo + ((hi - lo) >> 1);
-        if (chunk_sum[mid] <= goal) lo = mid;
-        else hi = mid;
+    int lo;
+    uint64_t rest;
+    if (staged) {
+        lo = last_not_above(g.chunks, goal, [&](int i) { return sums[i]; });
+        rest = goal - sums[lo];
+    } else {
+        lo = last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; });
+        rest = goal - chunk_sum[lo];
     }
-    const size_t c = (size_t)r * g.chunks + lo;
-    const uint64_t rest = goal - g.chunk_sum[c];
-    uint64_t tie_weight = 0;
-    uint32_t thr = 0, left = 0;                // ties of this chunk that are kept
-    if constexpr (CUT) {
-        thr = st.thr;
-        if (thr) {
-            tie_weight = st.tie_weight;
-            const uint32_t before = g.chunk_ties[c];
-            left = st.ties > before ? st.ties - before : 0u;
-        }
-    }
-    const uint64_t *seg_sum = g.seg_sum + c * kChunkThreads;
-    const uint32_t *seg_ties = CUT ? g.seg_ties + c * kChunkThreads : nullptr;
-    auto sum_before = [&](int i) {
-        uint64_t v = seg_sum[i];
-        if (CUT && thr) v += tie_weight * min(left, seg_ties[i]);
-        return v;
-    };
-    int sl = 0, sh = kChunkThreads;
-    while (sh - sl > 1) {
-        const int mid = (sl + sh) >> 1;
-        if (sum_before(mid) <= rest) sl = mid;
-        else sh = mid;
-    }
-    uint64_t run = sum_before(sl);
-    uint32_t rank = (CUT && thr) ? seg_ties[sl] : 0u;
+    const ChunkView<CUT> v(g, st, r, lo);
+    const int seg = last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); });
+    uint64_t run = v.sum_before(seg);
+    uint32_t rank = (CUT && v.thr) ? v.seg_ties[seg] : 0u;
     const char *row = row_base<DT>(a, r);
-    const int64_t i0 = (int64_t)lo * kChunk + (int64_t)sl * kSeg;
-    const uint32_t top = st.max_key;
-    const Scale s = scale_for<DT, OPACITY>(top, st.inv_t);
+    const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
+    const Scale s = st.scale;
     const double min_p = st.min_p;
-    int64_t id = -1;
+    uint32_t key[kSeg];
 #pragma unroll
     for (int q = 0; q < kSeg / kVec<DT>; q++) {
         uint32_t k[kVec<DT>];
         keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
-        for (int e = 0; e < kVec<DT>; e++) {
-            const bool tied = CUT && thr != 0 && k[e] == thr;
-            const bool keep = k[e] > thr || (tied && rank < left);
-            rank += tied;
-            if (id >= 0 || !keep || (greedy && k[e] != top)) continue;
-            const double w = weight<DT, OPACITY>(k[e], s);
-            if (w >= min_p) run += fixed(w, a.unit);
-            if (run > rest) id = i0 + q * kVec<DT> + e;
-        }
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
     }
-    ids[at] = (int32_t)id;
+    int id = -1;
+#pragma unroll
+    for (int e = 0; e < kSeg; e++) {
+        const bool tied = CUT && v.thr != 0 && key[e] == v.thr;
+        const bool keep = key[e] > v.thr || (tied && rank < v.left);
+        rank += tied;
+        if (id >= 0 || !keep || (greedy && key[e] != s.top)) continue;
+        const double w = weight<DT, OPACITY>(key[e], s);
+        if (w >= min_p) run += fixed(w, a.unit);
+        if (run > rest) id = e;
+    }
+    ids[at] = id < 0 ? -1 : (int32_t)(i0 + id);
+}
+
+// Few draws: a wave each, 64 running sums and then the 8 entries side by side; four dependent loads instead of twenty.
+template <int DT, bool OPACITY, bool CUT>
+__global__ void __launch_bounds__(64)
+k_long_draw_wave(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+    const int at = blockIdx.x, r = at / a.draws, lane = threadIdx.x;
+    const LongRow &st = g.rows[r];
+    const uint64_t total = st.total;
+    const float u = uniforms[at];
+    if (total == 0 || isnan(u)) {
+        if (lane == 0) ids[at] = -1;
+        return;
+    }
+    const bool greedy = st.greedy;
+    const uint64_t goal = greedy ? 0ull : goal_of(u, total);
+    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
+    const int lo = wave_last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; });
+    const uint64_t rest = goal - chunk_sum[lo];
+    const ChunkView<CUT> v(g, st, r, lo);
+    const int seg = wave_last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); });
+    const uint64_t before = v.sum_before(seg);
+    const uint32_t ties_before = (CUT && v.thr) ? v.seg_ties[seg] : 0u;
+    const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
+    uint32_t key = 0;
+    if (lane < kSeg && i0 + lane < a.cols) key = key_at<DT>(row_base<DT>(a, r), i0 + lane);
+    const bool tied = CUT && v.thr != 0 && key == v.thr;
+    const uint32_t rank =
+        ties_before + __builtin_popcountll(__builtin_amdgcn_ballot_w64(tied) & ((1ull << lane) - 1ull));
+    uint64_t mine = 0;
+    if ((key > v.thr || (tied && rank < v.left)) && (!greedy || key == st.scale.top)) {
+        const double w = weight<DT, OPACITY>(key, st.scale);
+        if (w >= st.min_p) mine = fixed(w, a.unit);
+    }
+    uint64_t run = mine;
+#pragma unroll
+    for (int off = 1; off < kSeg; off <<= 1) {
+        const uint64_t o = __shfl_up(run, off, 64);
+        if (lane >= off) run += o;
+    }
+    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < kSeg && before + run > rest);
+    if (lane == 0) ids[at] = over ? (int32_t)(i0 + __builtin_ctzll(over)) : -1;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 constexpr int kRowLimit = 8192;                // longest row of the one-workgroup form
 
 struct SampleLayout {
-    size_t rows, mass, count, chunk_max, chunk_sum, chunk_ties, seg_sum, seg_ties, total;
+    size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, seg_ties, total;
     int chunks;
     SampleLayout(int n_rows, int cols) {
         size_t o = 0;
@@ -841,13 +1066,14 @@ struct SampleLayout {
         chunks = cols > kRowLimit ? (int)(((int64_t)cols + kChunk - 1) / kChunk) : 0;
         const size_t n = (size_t)n_rows * chunks, some = chunks ? (size_t)n_rows : 0;
         rows = take(some * sizeof(LongRow));
-        mass = take(some * kBins * 8);
-        count = take(some * kBins * 4);
+        k_count = take(some * kLevels * kBins * 4);
+        p_mass = take(some * kLevels * kBins * 8);
+        p_count = take(some * kBins * 4);
         chunk_max = take(n * 4);
         chunk_sum = take(n * 8);
         chunk_ties = take(n * 4);
-        seg_sum = take(n * kChunkThreads * 8);
-        seg_ties = take(n * kChunkThreads * 4);
+        seg_sum = take(n * kChunkSegs * 8);
+        seg_ties = take(n * kChunkSegs * 4);
         total = o > 0 ? o : 256;
     }
 };
@@ -870,6 +1096,8 @@ static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids,
 // would grow with the square of the row.
 constexpr int kOwnMaxChunks = 4096;
 
+constexpr int64_t kWaveDraws = 8192;
+
 template <int DT, bool OPACITY, bool CUT>
 static int launch_long(const SampleArgs &a, const LongArgs &g, const float *uniforms, int32_t *ids, hipStream_t s) {
     const dim3 chunks((unsigned)((int64_t)a.rows * g.chunks)), rows(a.rows);
@@ -877,25 +1105,27 @@ static int launch_long(const SampleArgs &a, const LongArgs &g, const float *unif
     GS_LAUNCH_CHECK();
     const bool begun = CUT || g.chunks > kOwnMaxChunks;
     if (begun) {
-        GS_LAUNCH(k_long_begin, rows, dim3(kHistThreads), 0, s, a, g, CUT ? 1 : 0);
+        GS_LAUNCH((k_long_begin<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
         GS_LAUNCH_CHECK();
     }
     if constexpr (CUT) {
-        // two workgroups per compute unit over all the rows, and no part of a row below its first 8192 entries
-        const int64_t most = ((int64_t)a.cols + 8191) / 8192;
+        // two workgroups per compute unit over all the rows, none without a batch of loads
+        const int64_t batch = (int64_t)kHistThreads * kVec<DT> * kBatch, most = ((int64_t)a.cols + batch - 1) / batch;
         int64_t parts = (512 + a.rows - 1) / a.rows;
         if (parts > most) parts = most;
         const dim3 grid((unsigned)(parts * a.rows));
-        if (a.cfg.top_k_rows || a.cfg.top_k > 0)
+        if (g.with_k)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
                 GS_LAUNCH((k_long_digit<DT, OPACITY, false>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
                 GS_LAUNCH_CHECK();
             }
-        if (a.cfg.top_p_rows || a.cfg.top_p < 1.0f)
+        if (g.with_p)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
                 GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
                 GS_LAUNCH_CHECK();
             }
+        GS_LAUNCH((k_long_cut<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
+        GS_LAUNCH_CHECK();
     }
     if (begun) {
         GS_LAUNCH((k_long_sums<DT, OPACITY, CUT, true>), chunks, dim3(kChunkThreads), 0, s, a, g);
@@ -903,10 +1133,16 @@ static int launch_long(const SampleArgs &a, const LongArgs &g, const float *unif
         GS_LAUNCH((k_long_sums<DT, OPACITY, false, false>), chunks, dim3(kChunkThreads), 0, s, a, g);
     }
     GS_LAUNCH_CHECK();
-    GS_LAUNCH((k_long_scan<DT, OPACITY, CUT>), rows, dim3(kHistThreads), 0, s, a, g);
+    GS_LAUNCH((k_long_scan<CUT>), rows, dim3(kHistThreads), 0, s, g);
     GS_LAUNCH_CHECK();
-    const int64_t want = ((int64_t)a.rows * a.draws + 255) / 256;
-    GS_LAUNCH((k_long_draw<DT, OPACITY, CUT>), dim3((unsigned)want), dim3(256), 0, s, a, g, uniforms, ids);
+    // A wave per draw while the waves are all resident; at 64 rows of 131072 and one draw each 5 us against 10.
+    if ((int64_t)a.rows * a.draws <= kWaveDraws) {
+        GS_LAUNCH((k_long_draw_wave<DT, OPACITY, CUT>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g, uniforms, ids);
+    } else {
+        const int blocks = (a.draws + kDrawThreads - 1) / kDrawThreads;
+        const size_t lds = g.chunks <= kDrawChunks ? (size_t)g.chunks * 8 : 0;
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT>), dim3((unsigned)(blocks * a.rows)), dim3(kDrawThreads), lds, s, a, g, blocks, uniforms, ids);
+    }
     GS_LAUNCH_CHECK();
     return GS_OK;
 }
@@ -915,14 +1151,14 @@ template <int DT, bool OPACITY>
 static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *ids, char *ws, const SampleLayout &L,
                          hipStream_t s) {
     if (L.chunks == 0) return launch_rows<DT, OPACITY>(a, uniforms, ids, s);
-    const LongArgs g = {(LongRow *)(ws + L.rows), (uint64_t *)(ws + L.mass), (uint32_t *)(ws + L.count),
-                        (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
-                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint32_t *)(ws + L.seg_ties),
-                        L.chunks};
     const GsSampleConfig &c = a.cfg;
-    const bool cut = c.top_k_rows || c.top_k > 0 || c.top_p_rows || c.top_p < 1.0f;
-    return cut ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
-               : launch_long<DT, OPACITY, false>(a, g, uniforms, ids, s);
+    const bool with_k = c.top_k_rows || c.top_k > 0, with_p = c.top_p_rows || c.top_p < 1.0f;
+    const LongArgs g = {(LongRow *)(ws + L.rows), (uint32_t *)(ws + L.k_count), (uint64_t *)(ws + L.p_mass),
+                        (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
+                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint32_t *)(ws + L.seg_ties),
+                        L.chunks, with_k, with_p};
+    return with_k || with_p ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
+                            : launch_long<DT, OPACITY, false>(a, g, uniforms, ids, s);
 }
 
 }  // namespace gs
@@ -948,7 +1184,7 @@ extern "C" int gs_sample(int rows, int cols, const void *logits, int64_t row_str
         return GS_ERR_INVALID_ARGUMENT;
     const SampleLayout L(rows, cols);
     // a launch's workgroups, 31 bits
-    if (((int64_t)rows * draws + 255) / 256 > 0x7fffffffLL || (int64_t)rows * L.chunks > 0x7fffffffLL)
+    if ((int64_t)rows * (((int64_t)draws + kDrawThreads - 1) / kDrawThreads) > 0x7fffffffLL || (int64_t)rows * L.chunks > 0x7fffffffLL)
         return GS_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < L.total) return GS_ERR_WORKSPACE;
     SampleArgs a = {logits, row_stride, rows, cols, draws, 0.0, *cfg};

@@ -990,7 +990,7 @@ Tensor TileBalance::forward(AutogradContext *ctx, Tensor opacities, Tensor packe
     const bool want = opacities.requires_grad();
     Tensor loss = torch::empty({}, packed.options());
     Tensor v = want ? torch::empty(opacities.sizes(), packed.options()) : Tensor();
-    const size_t bytes = gs_tile_balance_workspace_bytes((int)imgWidth, (int)imgHeight);
+    const size_t bytes = gs_tile_balance_workspace_bytes((int)imgWidth, (int)imgHeight, (int)N);
     Tensor ws = torch::empty({(int64_t)bytes}, packed.options().dtype(torch::kUInt8));
     check_status(gs_tile_balance((int)imgWidth, (int)imgHeight, (int)N, fptr(packed), tileBins.data_ptr<int32_t>(), 1.0f,
                                  fptr_mut(loss), nullptr, want ? fptr_mut(v) : nullptr,

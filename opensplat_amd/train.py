@@ -256,7 +256,7 @@ class Trainer:
         dev = self.dev
         tiles = ((W + cabi.GS_TILE - 1) // cabi.GS_TILE) * ((H + cabi.GS_TILE - 1) // cabi.GS_TILE)
         return (torch.empty(1, device=dev), torch.empty(tiles, device=dev, dtype=torch.int32), self.grads.v_opacity), \
-            torch.empty(cabi.lib().gs_tile_balance_workspace_bytes(W, H), device=dev, dtype=torch.uint8)
+            torch.empty(cabi.lib().gs_tile_balance_workspace_bytes(W, H, self.N), device=dev, dtype=torch.uint8)
 
     def _balance(self, W, H, b, scale, out, workspace):
         """The balance loss of the frame's lists, its gradient added to the opacities' (behind gaussian_backward)."""

@@ -204,7 +204,7 @@ def close(got, want, operands):
 
 
 @pytest.mark.parametrize("shape", [(1, 16, 16), (1, 1, 1), (7, 17, 33), (300, 100, 50), (2000, 640, 360), (500, 4111, 20),
-                                   (500, 20, 4111), (3000, 1920, 1080)])
+                                   (500, 20, 4111), (3000, 1920, 1080), (2000, 9999, 1050), (700, 40000, 300)])
 @pytest.mark.parametrize("logit", [False, True])
 def test_tile_balance(shape, logit):
     from opensplat_amd import cabi

@@ -53,9 +53,10 @@ def test_tile_balance_refuses(kw):
 
 def test_tile_balance_limits():
     assert balance(W=65536) == UNSUPPORTED and balance(H=65536) == UNSUPPORTED
-    need = cabi.lib().gs_tile_balance_workspace_bytes(64, 64)
+    need = cabi.lib().gs_tile_balance_workspace_bytes(64, 64, 4)
     assert need > 0 and balance(size=need - 1) == WORKSPACE
-    assert cabi.lib().gs_tile_balance_workspace_bytes(0, 5) == 0
+    assert cabi.lib().gs_tile_balance_workspace_bytes(0, 5, 4) == 0 and \
+        cabi.lib().gs_tile_balance_workspace_bytes(64, 64, -1) == 0
 
 
 def relocate(N=9, K=4, pairs=2, targets=ONE, sources=ONE, low=0.005, params=True, ws=ONE, size=BIG, drop=()):
