@@ -145,6 +145,44 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class _on:
+    """The device of a call's tensors as the current one, for calls whose kernels are as short as the host's part of
+    them: nothing to enter or leave where it is the current one already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _raw_stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+_ws_sizes = {}
+
+
+def _workspace(workspace, dev, fn, *sizes):
+    """The caller's workspace, or one of the bytes that `fn` names for these sizes."""
+    need = _ws_sizes.get((fn, sizes))
+    if need is None:
+        if len(_ws_sizes) > 4096:
+            _ws_sizes.clear()
+        need = _ws_sizes[fn, sizes] = max(int(getattr(lib(), fn)(*sizes)), 16)
+    if workspace is None:
+        return torch.empty(need, device=dev, dtype=torch.uint8)
+    if workspace.numel() * workspace.element_size() < need or workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, of at least %d bytes, on %s" % (need, dev))
+    return workspace
+
+
 def make_camera(viewmat, projmat, fx, fy, cx, cy, W, H, clip=0.01, glob_scale=1.0,
                 flags=0) -> GsCamera:
     cam = GsCamera()
@@ -679,27 +717,31 @@ def tile_balance(W, H, packed, tile_bins, scale=1.0, flags=0, want_grad=True, ou
     opacity of tile t's list.  packed [N, 12] and tile_bins [T, 2]: the frame's binning (Binned.packed, .tile_bins).
     flags: GS_FLAG_LOGIT_OPACITY (gradient w.r.t. the logits), GS_FLAG_ACCUMULATE_GRADS (needs out).
     -> (loss [1], counts [T] int32, v_opacity [N] or None)."""
-    dev = packed.device
-    N, tiles = packed.shape[0], ((W + GS_TILE - 1) // GS_TILE) * ((H + GS_TILE - 1) // GS_TILE)
-    if packed.dtype != torch.float32 or packed.shape != (N, GS_SPLAT_DWORDS):
-        raise ValueError("packed must be float32 [N, %d]" % GS_SPLAT_DWORDS)
-    if tile_bins.dtype != torch.int32 or tile_bins.shape != (tiles, 2) or tile_bins.device != dev:
-        raise ValueError("tile_bins must be int32 [%d, 2] on %s" % (tiles, dev))
+    dev, tiles = packed.device, -(-W // GS_TILE) * -(-H // GS_TILE)
+    if not packed.is_cuda or packed.dtype != torch.float32 or packed.dim() != 2 or packed.shape[1] != GS_SPLAT_DWORDS \
+            or not packed.is_contiguous():
+        raise ValueError("packed must be contiguous float32 [N, %d] on the GPU" % GS_SPLAT_DWORDS)
+    if tile_bins.dtype != torch.int32 or tile_bins.shape != (tiles, 2) or tile_bins.device != dev \
+            or not tile_bins.is_contiguous():
+        raise ValueError("tile_bins must be contiguous int32 [%d, 2] on %s" % (tiles, dev))
+    N = packed.shape[0]
     if out is None:
         if flags & GS_FLAG_ACCUMULATE_GRADS:
             raise ValueError("GS_FLAG_ACCUMULATE_GRADS adds to a v_opacity of the caller's: pass out")
-        out = (torch.empty(1, device=dev, dtype=torch.float32), torch.empty(tiles, device=dev, dtype=torch.int32),
-               torch.empty(N, device=dev, dtype=torch.float32) if want_grad else None)
-    loss, counts, v = out
-    for t, n, dt in ((loss, 1, torch.float32), (counts, tiles, torch.int32), (v, N, torch.float32)):
-        if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev):
-            raise ValueError("out must be (float32 [1], int32 [%d], float32 [%d]) on %s" % (tiles, N, dev))
-    with torch.cuda.device(dev):
-        need = lib().gs_tile_balance_workspace_bytes(W, H, N)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-        _check(lib().gs_tile_balance(W, H, N, _p(packed), _p(tile_bins), scale, _p(loss), _p(counts), _p(v), flags,
-                                     _p(workspace), workspace.numel(), _stream()), "gs_tile_balance")
+        loss, counts = torch.empty(1, device=dev, dtype=torch.float32), torch.empty(tiles, device=dev, dtype=torch.int32)
+        v = torch.empty(N, device=dev, dtype=torch.float32) if want_grad else None
+    else:
+        loss, counts, v = out
+        for t, n, dt in ((loss, 1, torch.float32), (counts, tiles, torch.int32), (v, N, torch.float32)):
+            if t is not None and (t.numel() != n or t.dtype != dt or t.device != dev or not t.is_contiguous()):
+                raise ValueError("out must be contiguous (float32 [1], int32 [%d], float32 [%d]) on %s" % (tiles, N, dev))
+    with _on(dev):
+        ws = _workspace(workspace, dev, "gs_tile_balance_workspace_bytes", W, H, N)
+        rc = lib().gs_tile_balance(W, H, N, packed.data_ptr(), tile_bins.data_ptr(), scale, loss.data_ptr(),
+                                   None if counts is None else counts.data_ptr(), None if v is None else v.data_ptr(),
+                                   flags, ws.data_ptr(), ws.numel() * ws.element_size(), _raw_stream(dev))
+    if rc:
+        _check(rc, "gs_tile_balance")
     return loss, counts, v
 
 
@@ -820,43 +862,46 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
     if not logits.is_cuda:
         raise ValueError("logits must be on the GPU")
     dev, shape = logits.device, uniforms.shape
-    if logits.dim() == 1:
-        logits = logits[None]
-    if uniforms.dim() == 1:
-        uniforms = uniforms[None]
-    if logits.dim() != 2 or uniforms.dim() != 2 or uniforms.shape[0] != logits.shape[0]:
+    if logits.dim() == 2 and uniforms.dim() == 2 and shape[0] == logits.shape[0]:
+        R, V = logits.shape
+        stride, entry = logits.stride()
+    elif logits.dim() == 1 and uniforms.dim() == 1:
+        R, V = 1, logits.shape[0]
+        stride, entry = V, logits.stride(0)
+    else:
         raise ValueError("logits [R, V] and uniforms [R, D] (or [V] and [D]) needed, got %s and %s"
                          % (tuple(logits.shape), tuple(shape)))
-    R, V = logits.shape
-    if logits.dtype not in _SAMPLE_DTYPES:
+    dtype = _SAMPLE_DTYPES.get(logits.dtype)
+    if dtype is None:
         raise ValueError("logits must be float32, float16 or bfloat16, not %s" % logits.dtype)
-    if V > 1 and logits.stride(1) != 1:
+    if V > 1 and entry != 1:
         raise ValueError("the entries of a row must be adjacent (stride 1)")
-    if R > 1 and logits.stride(0) < V:
+    if R > 1 and stride < V:
         raise ValueError("rows of the logits must not overlap")
     if uniforms.dtype != torch.float32 or uniforms.device != dev or not uniforms.is_contiguous():
         raise ValueError("uniforms must be contiguous float32 on %s" % dev)
-    cfg = GsSampleConfig(_SAMPLE_DTYPES[logits.dtype], GS_FLAG_LOGIT_OPACITY if opacity else 0, 1.0, 0, 1.0, 0.0)
+    cfg = GsSampleConfig(dtype, GS_FLAG_LOGIT_OPACITY if opacity else 0, 1.0, 0, 1.0, 0.0)
     for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if v is None:
+            continue
         if isinstance(v, torch.Tensor):
             if v.shape != (R,) or v.device != dev or not v.is_contiguous() or \
                     v.dtype != (torch.int32 if name == "top_k" else torch.float32):
                 raise ValueError("%s must be a number or a contiguous %s tensor [%d] on %s"
                                  % (name, "int32" if name == "top_k" else "float32", R, dev))
             setattr(cfg, name + "_rows", v.data_ptr())
-        elif v is not None:
+        else:
             setattr(cfg, name, v)
     if out is None:
         out = torch.empty(shape, device=dev, dtype=torch.int32)
     elif out.shape != shape or out.dtype != torch.int32 or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous int32 %s on %s" % (tuple(shape), dev))
-    with torch.cuda.device(dev):
-        need = lib().gs_sample_workspace_bytes(R, V)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
-        _check(lib().gs_sample(R, V, logits.data_ptr(), logits.stride(0) if R > 1 else V, C.byref(cfg),
-                               uniforms.shape[1], _p(uniforms), _p(out), _p(workspace), workspace.numel(), _stream()),
-               "gs_sample")
+    with _on(dev):
+        ws = _workspace(workspace, dev, "gs_sample_workspace_bytes", R, V)
+        rc = lib().gs_sample(R, V, logits.data_ptr(), stride if R > 1 else V, C.byref(cfg), shape[-1], uniforms.data_ptr(),
+                             out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), _raw_stream(dev))
+    if rc:
+        _check(rc, "gs_sample")
     return out
 
 
@@ -866,29 +911,36 @@ def relocate(params, exp_avg, exp_avg_sq, targets, sources, min_opacity=0.005, w
     exp_avg_sq: lists of the six tensors [means, log_scales, quats, opacity_logits, features_dc, features_rest] (the
     moment lists may be None).  Pairs with an index outside [0, N) change nothing, as do pairs whose source is a target
     and all but the first pair of a target."""
-    means, dev = params[0], params[0].device
-    N, n = means.shape[0], targets.numel()
+    dev, N, n = params[0].device, params[0].shape[0], targets.numel()
     rest = params[5] if len(params) > 5 else None
     K = 1 + (rest.shape[1] if rest is not None and rest.numel() > 0 else 0)
     for t in (targets, sources):
         if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != dev or not t.is_contiguous():
             raise ValueError("targets and sources must be contiguous int32 [n] on %s" % dev)
     lens = (3, 3, 4, 1, 3, 3 * (K - 1))
+    sets = []
     for tensors in (params, exp_avg, exp_avg_sq):
-        for t, k in zip(tensors or (), lens):
-            if t is not None and (t.numel() != N * k or t.device != dev):
-                raise ValueError("a Gaussian set of %d rows and K = %d needs tensors of %s floats a row on %s"
-                                 % (N, K, lens, dev))
+        if not tensors:
+            sets.append(None)
+            continue
+        at = [0] * 6
+        for i, t in enumerate(tensors):
+            if t is None:
+                continue
+            if not t.is_cuda or t.numel() != N * lens[i] or t.dtype != torch.float32 or t.device != dev \
+                    or not t.is_contiguous():
+                raise ValueError("a Gaussian set of %d rows and K = %d needs contiguous float32 tensors of %s floats a row "
+                                 "on %s" % (N, K, lens, dev))
+            at[i] = t.data_ptr() if lens[i] else 0
+        sets.append(C.byref(GsGaussianSet(*at)))
     if N == 0 or n == 0:
         return
-    with torch.cuda.device(dev):
-        need = lib().gs_relocate_workspace_bytes(N, n)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-        sets = [_set(t) if t else None for t in (params, exp_avg, exp_avg_sq)]
-        _check(lib().gs_relocate(N, K, n, _p(targets), _p(sources), min_opacity,
-                                 *[C.byref(s) if s is not None else None for s in sets], _p(workspace),
-                                 workspace.numel(), _stream()), "gs_relocate")
+    with _on(dev):
+        ws = _workspace(workspace, dev, "gs_relocate_workspace_bytes", N, n)
+        rc = lib().gs_relocate(N, K, n, targets.data_ptr(), sources.data_ptr(), min_opacity, *sets, ws.data_ptr(),
+                               ws.numel() * ws.element_size(), _raw_stream(dev))
+    if rc:
+        _check(rc, "gs_relocate")
 
 
 # ---------------------------------------------------------------------------------------------

@@ -107,8 +107,20 @@ static __device__ __forceinline__ double block_sum_f64(double v, double *red /* 
     return r;
 }
 
+// Inclusive sum over the wave's lanes without LDS: shifts by 1, 2, 4, 8 inside rows of 16, then each row's last lane into
+// the next row, then lane 31 into the upper half.
+static __device__ __forceinline__ int32_t wave_scan(int32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 constexpr int kSumThreads = 1024;
-constexpr int kSumParts = 512;                 // workgroups at most: two per compute unit
+constexpr int kSumParts = 256;                 // workgroups at most: one per compute unit
 constexpr int kColParts = 4;
 
 // The summed-area table of the lists' lengths in LDS.  A wave scans a tile row; a column is scanned in four parts, whose
@@ -116,10 +128,10 @@ constexpr int kColParts = 4;
 static __device__ __forceinline__ void lds_table(const BalanceGrid &g, const int2 *__restrict__ bins,
                                                  int32_t *__restrict__ counts, int32_t *table, int32_t *part_sum) {
     const int tid = threadIdx.x, lane = tid & 63, tiles = g.tw * g.th;
-    for (int i0 = 0; i0 < tiles; i0 += 4 * kSumThreads) {
-        int32_t n[4];
+    for (int i0 = 0; i0 < tiles; i0 += 8 * kSumThreads) {
+        int32_t n[8];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 8; k++) {
             const int i = i0 + k * kSumThreads + tid;
             n[k] = 0;
             if (i < tiles) {
@@ -128,7 +140,7 @@ static __device__ __forceinline__ void lds_table(const BalanceGrid &g, const int
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 8; k++) {
             const int i = i0 + k * kSumThreads + tid;
             if (i < tiles) {
                 const int y = i / g.tw, x = i - y * g.tw;
@@ -144,12 +156,7 @@ static __device__ __forceinline__ void lds_table(const BalanceGrid &g, const int
         int32_t base = 0;
         for (int x0 = 1; x0 <= g.tw; x0 += 64) {
             const int x = x0 + lane;
-            int32_t s = x <= g.tw ? table[y * g.pitch + x] : 0;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int32_t o = __shfl_up(s, off, 64);
-                if (lane >= off) s += o;
-            }
+            const int32_t s = wave_scan(x <= g.tw ? table[y * g.pitch + x] : 0);
             if (x <= g.tw) table[y * g.pitch + x] = base + s;
             base += __builtin_amdgcn_readlane(s, 63);
         }
@@ -186,39 +193,49 @@ k_balance_sums(BalanceGrid g, int N, const float *__restrict__ packed, const int
     __shared__ double red[kSumThreads / 64];
     __shared__ int32_t part_sum[kSumThreads];
     extern __shared__ int32_t table_lds[];
+    // Four records a thread are under way at a time: the first while the table is made, the next while these are looked up.
+    struct Batch {
+        float o[4];
+        uint32_t rx[4], ry[4];
+    };
+    const int64_t stride = (int64_t)gridDim.x * kSumThreads;
+    auto load = [&](int64_t n0) {
+        Batch b;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t n = n0 + k * stride;
+            b.rx[k] = b.ry[k] = 0;
+            b.o[k] = 0.0f;
+            if (n < N) {
+                const float *p = packed + (size_t)n * GS_SPLAT_DWORDS;
+                b.o[k] = p[5];
+                b.rx[k] = __float_as_uint(p[7]);
+                b.ry[k] = __float_as_uint(p[11]);
+            }
+        }
+        return b;
+    };
+    int64_t n0 = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
+    Batch next = load(n0);
     const int32_t *table = table_mem;
     if constexpr (LDS) {
         lds_table(g, bins, blockIdx.x == 0 ? counts : nullptr, table_lds, part_sum);
         table = table_lds;
     }
     double q = 0.0, s = 0.0;
-    const int64_t stride = (int64_t)gridDim.x * kSumThreads;
-    for (int64_t n0 = (int64_t)blockIdx.x * kSumThreads + threadIdx.x; n0 < N; n0 += 4 * stride) {
-        // (four records' loads under way together)
-        float o[4];
-        uint32_t rx[4], ry[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int64_t n = n0 + k * stride;
-            rx[k] = ry[k] = 0;
-            o[k] = 0.0f;
-            if (n < N) {
-                const float *p = packed + (size_t)n * GS_SPLAT_DWORDS;
-                o[k] = p[5];
-                rx[k] = __float_as_uint(p[7]);
-                ry[k] = __float_as_uint(p[11]);
-            }
-        }
+    for (; n0 < N; n0 += 4 * stride) {
+        const Batch b = next;
+        next = load(n0 + 4 * stride);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int64_t n = n0 + k * stride;
             if (n >= N) continue;
-            const Cover c = cover_of(g, table, rx[k], ry[k]);
+            const Cover c = cover_of(g, table, b.rx[k], b.ry[k]);
             cover[n] = make_int2(c.entries, c.tiles);
-            opacity[n] = o[k];
+            opacity[n] = b.o[k];
             if (c.tiles > 0) {
-                q += (double)o[k] * (double)c.entries;
-                s += (double)o[k] * (double)c.tiles;
+                q += (double)b.o[k] * (double)c.entries;
+                s += (double)b.o[k] * (double)c.tiles;
             }
         }
     }
@@ -248,20 +265,29 @@ k_balance_grad(BalanceGrid g, int N, int nparts, const double2 *__restrict__ par
     if (blockIdx.x == 0 && threadIdx.x == 0) loss[0] = (float)(scale * (norm * mean));
     if (!v_opacity) return;
     const double k = some ? scale * norm / s : 0.0;
-    for (int64_t n = (int64_t)blockIdx.x * kBalThreads + threadIdx.x; n < N; n += (int64_t)gridDim.x * kBalThreads) {
-        const int2 c = cover[n];
-        double v = 0.0;
-        if (some && c.y > 0) {
-            v = k * ((double)c.x - (double)c.y * mean);
-            if (flags & GS_FLAG_LOGIT_OPACITY) {
-                const double o = (double)opacity[n];
-                v *= o * (1.0 - o);
-            }
-        }
-        if (flags & GS_FLAG_ACCUMULATE_GRADS) {
-            if (c.y > 0) v_opacity[n] += (float)v;
+    auto slope = [&](int entries_, int tiles, float op) {
+        if (!some || tiles <= 0) return 0.0f;
+        double v = k * ((double)entries_ - (double)tiles * mean);
+        if (flags & GS_FLAG_LOGIT_OPACITY) v *= (double)op * (1.0 - (double)op);
+        return (float)v;
+    };
+    const bool add = flags & GS_FLAG_ACCUMULATE_GRADS;
+    const int64_t step = (int64_t)gridDim.x * kBalThreads * 4;
+    for (int64_t n = ((int64_t)blockIdx.x * kBalThreads + threadIdx.x) * 4; n < N; n += step) {
+        // (the workspace's arrays are padded to whole fours; v_opacity may have any alignment of a float)
+        const int4 c0 = *reinterpret_cast<const int4 *>(cover + n), c1 = *reinterpret_cast<const int4 *>(cover + n + 2);
+        const float4 op = *reinterpret_cast<const float4 *>(opacity + n);
+        const float v[4] = {slope(c0.x, c0.y, op.x), slope(c0.z, c0.w, op.y), slope(c1.x, c1.y, op.z), slope(c1.z, c1.w, op.w)};
+        const bool in[4] = {c0.y > 0, c0.w > 0, c1.y > 0, c1.w > 0};
+        if (!add && n + 4 <= N) {
+            __builtin_memcpy(v_opacity + n, v, 16);
         } else {
-            v_opacity[n] = (float)v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (n + e >= N) break;
+                if (!add) v_opacity[n + e] = v[e];
+                else if (in[e]) v_opacity[n + e] += v[e];
+            }
         }
     }
 }
@@ -284,8 +310,8 @@ struct BalanceLayout {
         table = take(lds ? 0 : table_bytes);
         parts = take((size_t)kSumParts * sizeof(double2));
         entries = take(sizeof(int32_t));
-        cover = take((size_t)N * sizeof(int2));
-        opacity = take((size_t)N * sizeof(float));
+        cover = take(((size_t)N + 3) * sizeof(int2));
+        opacity = take(((size_t)N + 3) * sizeof(float));
         total = o;
     }
 };
@@ -319,12 +345,13 @@ extern "C" int gs_tile_balance(int W, int H, int N, const float *packed, const i
     float *opacity = (float *)(ws + L.opacity);
     hipStream_t s = (hipStream_t)stream;
     const int2 *bins = (const int2 *)tile_bins;
-    // at least 1024 Gaussians a workgroup; a table beyond half of the LDS leaves room for one workgroup per compute unit
-    const int64_t want = ((int64_t)N + kSumThreads - 1) / kSumThreads, most = L.lds && L.table_bytes > 70 * 1024 ? 256 : kSumParts;
+    // one Gaussian a thread at least
+    const int64_t want = ((int64_t)N + kSumThreads - 1) / kSumThreads, most = kSumParts;
     const int blocks = (int)(want < 1 ? 1 : (want < most ? want : most));
     if (L.lds) {
-        GS_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(k_balance_sums<true>),
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLdsTable));
+        if (L.table_bytes > 48 * 1024)         // (beyond what every launch may have)
+            GS_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(k_balance_sums<true>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLdsTable));
         GS_LAUNCH((k_balance_sums<true>), dim3(blocks), dim3(kSumThreads), L.table_bytes, s, L.g, N, packed, bins, counts,
                   (const int32_t *)nullptr, cover, opacity, parts, entries);
     } else {
@@ -336,8 +363,8 @@ extern "C" int gs_tile_balance(int W, int H, int N, const float *packed, const i
                   opacity, parts, entries);
     }
     GS_LAUNCH_CHECK();
-    const int64_t grads = v_opacity ? ((int64_t)N + kBalThreads - 1) / kBalThreads : 1;
-    GS_LAUNCH(k_balance_grad, dim3((unsigned)(grads < 1 ? 1 : (grads < 4096 ? grads : 4096))), dim3(kBalThreads), 0, s, L.g, N,
+    const int64_t grads = v_opacity ? ((int64_t)N + 4 * kBalThreads - 1) / (4 * kBalThreads) : 1;
+    GS_LAUNCH(k_balance_grad, dim3((unsigned)(grads < 1 ? 1 : (grads < 1024 ? grads : 1024))), dim3(kBalThreads), 0, s, L.g, N,
               blocks, parts, entries, cover, opacity, (double)scale, flags, loss, v_opacity);
     GS_LAUNCH_CHECK();
     return GS_OK;

@@ -78,6 +78,51 @@ k_relocate_count(int N, int pairs, const int32_t *__restrict__ targets, const in
     out[i] = p;
 }
 
+// The three of them for few pairs, as one workgroup's phases (launches of a microsecond of work cost the host two each).
+// The words pass through the device's atomics: a load of this unit's own cache could be older.
+constexpr int kFewPairs = 2048;
+__global__ void __launch_bounds__(1024)
+k_relocate_few(int N, int pairs, const int32_t *__restrict__ targets, const int32_t *__restrict__ sources, int32_t *owner,
+               int32_t *copies, const float *__restrict__ logits, const float *__restrict__ log_scales,
+               RelocatePair *__restrict__ out) {
+    int32_t t[kFewPairs / 1024], s[kFewPairs / 1024];
+#pragma unroll
+    for (int k = 0; k < kFewPairs / 1024; k++) {
+        const int i = k * 1024 + threadIdx.x;
+        t[k] = s[k] = -1;
+        if (i < pairs) {
+            t[k] = targets[i];
+            s[k] = sources[i];
+        }
+        if (in_range(t[k], N) && in_range(s[k], N)) {
+            __hip_atomic_store(&owner[t[k]], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&owner[s[k]], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&copies[s[k]], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        } else {
+            t[k] = -1;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kFewPairs / 1024; k++)
+        if (t[k] >= 0) atomicMin(&owner[t[k]], k * 1024 + (int)threadIdx.x);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kFewPairs / 1024; k++) {
+        const int i = k * 1024 + threadIdx.x;
+        RelocatePair p = {0.0f, 0.0f, 0.0f, 0.0f, -1};
+        if (t[k] >= 0 && __hip_atomic_load(&owner[t[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i &&
+            __hip_atomic_load(&owner[s[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kNoOwner) {
+            p.logit = logits[s[k]];
+            p.s0 = log_scales[3 * (size_t)s[k]];
+            p.s1 = log_scales[3 * (size_t)s[k] + 1];
+            p.s2 = log_scales[3 * (size_t)s[k] + 2];
+            p.rank = atomicAdd(&copies[s[k]], 1);
+        }
+        if (i < pairs) out[i] = p;
+    }
+}
+
 struct RelocateSets {
     float *p[6], *m[6], *v[6];
     int columns;                               // floats per Gaussian over the six tensors
@@ -211,13 +256,19 @@ extern "C" int gs_relocate(int N, int K, int pairs, const int32_t *targets, cons
     RelocatePair *held = (RelocatePair *)(ws + L.pairs_off);
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid((pairs + kRelThreads - 1) / kRelThreads), block(kRelThreads);
-    GS_LAUNCH(k_relocate_clear, grid, block, 0, s, N, pairs, targets, sources, owner, copies);
-    GS_LAUNCH_CHECK();
-    GS_LAUNCH(k_relocate_claim, grid, block, 0, s, N, pairs, targets, sources, owner);
-    GS_LAUNCH_CHECK();
-    GS_LAUNCH(k_relocate_count, grid, block, 0, s, N, pairs, targets, sources, owner, copies, p.opacity_logits,
-              p.log_scales, held);
-    GS_LAUNCH_CHECK();
+    if (pairs <= kFewPairs) {
+        GS_LAUNCH(k_relocate_few, dim3(1), dim3(1024), 0, s, N, pairs, targets, sources, owner, copies, p.opacity_logits,
+                  p.log_scales, held);
+        GS_LAUNCH_CHECK();
+    } else {
+        GS_LAUNCH(k_relocate_clear, grid, block, 0, s, N, pairs, targets, sources, owner, copies);
+        GS_LAUNCH_CHECK();
+        GS_LAUNCH(k_relocate_claim, grid, block, 0, s, N, pairs, targets, sources, owner);
+        GS_LAUNCH_CHECK();
+        GS_LAUNCH(k_relocate_count, grid, block, 0, s, N, pairs, targets, sources, owner, copies, p.opacity_logits,
+                  p.log_scales, held);
+        GS_LAUNCH_CHECK();
+    }
     RelocateSets a = {{p.means, p.log_scales, p.quats, p.opacity_logits, p.features_dc, p.features_rest},
                       {m.means, m.log_scales, m.quats, m.opacity_logits, m.features_dc, m.features_rest},
                       {v.means, v.log_scales, v.quats, v.opacity_logits, v.features_dc, v.features_rest},
