@@ -117,28 +117,31 @@ static __device__ __forceinline__ void keys_at(const char *row, int64_t i, int64
 }
 
 // ---- weights ----------------------------------------------------------------------------------------------------
-// 2^y for y <= 0 by 2^n times the Taylor polynomial of 2^f, |f| <= 1/2: (ln 2 / 2)^13 / 13! = 2e-16.  Adding 1.5 2^52
-// rounds y to the integer n and leaves n in the low word; it goes into the exponent by an integer addition (the slower
-// rint, ldexp and conversions cost as much as the polynomial).  Below 2^-1000: 2^-1000.
+// p * x + c with the constant in scalar registers: left to itself the compiler takes the two-address form and copies every
+// coefficient of a polynomial into vector registers first, one instruction in six of a weight.
+static __device__ __forceinline__ double fma_const(double p, double x, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(p), "v"(x), "s"(c));
+    return r;
+}
+
+// 2^y for y <= 0: 2^n times the polynomial that agrees with 2^f at the eleven Chebyshev nodes of |f| <= 1/2 (3e-16
+// relative).  Adding 1.5 2^52 rounds y to the integer n and leaves n in the low word; it goes into the exponent by an
+// integer addition.  Below 2^-1000: 2^-1000.
 static __device__ __forceinline__ double pow2(double y) {
     y = fmax(y, -1000.0);
     const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
     const int n = (int)(uint32_t)__double_as_longlong(shifted);
-    constexpr double L = 0.69314718055994530941723212145818;
-    constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
-                     c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11,
-                     c12 = c11 * L / 12;
-    double p = fma(c12, f, c11);
-    p = fma(p, f, c10);
-    p = fma(p, f, c9);
-    p = fma(p, f, c8);
-    p = fma(p, f, c7);
-    p = fma(p, f, c6);
-    p = fma(p, f, c5);
-    p = fma(p, f, c4);
-    p = fma(p, f, c3);
-    p = fma(p, f, c2);
-    p = fma(p, f, c1);
+    double p = 0x1.e6063f7217bc6p-28;
+    p = fma_const(p, f, 0x1.b675bca4eeebbp-24);
+    p = fma_const(p, f, 0x1.62bfd47773353p-20);
+    p = fma_const(p, f, 0x1.ffcb54062e698p-17);
+    p = fma_const(p, f, 0x1.430913096fd9fp-13);
+    p = fma_const(p, f, 0x1.5d87fe9d7a584p-10);
+    p = fma_const(p, f, 0x1.3b2ab6fba1ddap-7);
+    p = fma_const(p, f, 0x1.c6b08d703ce49p-5);
+    p = fma_const(p, f, 0x1.ebfbdff82c598p-3);
+    p = fma_const(p, f, 0x1.62e42fefa3a19p-1);
     p = fma(p, f, 1.0);
     return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
 }
@@ -149,24 +152,20 @@ static __device__ __forceinline__ double reciprocal(double d) {   // d in [1, 2]
     r = fma(fma(-d, r, 1.0), r, r);
     return fma(fma(-d, r, 1.0), r, r);
 }
-// log(1 + z), z in [0, 1]: 2 atanh(s) with s = z / (2 + z) <= 1/3; (1/9)^16 / 33 = 2e-17
+// log(1 + z), z in [0, 1]: 2 atanh(s) = 2 s (1 + q h(q)) with s = z / (2 + z) <= 1/3, q = s^2, and h by its polynomial
+// through ten Chebyshev nodes of [0, 1/9] (2e-16 relative, of which q h passes on a twenty-fifth)
 static __device__ __forceinline__ double log1p_unit(double z) {
     const double s = z * reciprocal(2.0 + z), q = s * s;
-    double p = 1.0 / 31;
-    p = fma(p, q, 1.0 / 29);
-    p = fma(p, q, 1.0 / 27);
-    p = fma(p, q, 1.0 / 25);
-    p = fma(p, q, 1.0 / 23);
-    p = fma(p, q, 1.0 / 21);
-    p = fma(p, q, 1.0 / 19);
-    p = fma(p, q, 1.0 / 17);
-    p = fma(p, q, 1.0 / 15);
-    p = fma(p, q, 1.0 / 13);
-    p = fma(p, q, 1.0 / 11);
-    p = fma(p, q, 1.0 / 9);
-    p = fma(p, q, 1.0 / 7);
-    p = fma(p, q, 1.0 / 5);
-    p = fma(p, q, 1.0 / 3);
+    double p = 0x1.4b0a26c5f2aefp-4;
+    p = fma_const(p, q, 0x1.687a6e7c95176p-5);
+    p = fma_const(p, q, 0x1.eb905e8575054p-5);
+    p = fma_const(p, q, 0x1.10ac75dc602b1p-4);
+    p = fma_const(p, q, 0x1.3b18b294bebf9p-4);
+    p = fma_const(p, q, 0x1.745cf0b0e03bdp-4);
+    p = fma_const(p, q, 0x1.c71c727143318p-4);
+    p = fma_const(p, q, 0x1.24924923d44c6p-3);
+    p = fma_const(p, q, 0x1.999999999a3ddp-3);
+    p = fma_const(p, q, 0x1.5555555555555p-2);
     return 2.0 * fma(p * q, s, s);
 }
 template <bool OPACITY>
@@ -881,17 +880,24 @@ k_long_scan(LongArgs g) {
     if (tid == 0) st.total = ok ? base : 0ull;
 }
 
-// The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not exceed `goal`; four-fold steps, whose three
-// loads are under way together.
+// The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not exceed `goal`, and that value; four-fold steps,
+// whose three loads are under way together.
 template <typename F>
-static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f) {
+static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f, uint64_t &at_lo) {
     int lo = 0;
+    at_lo = 0;
     while (n > 1) {
         const int step = (n + 3) >> 2;
         uint64_t v[3];
 #pragma unroll
         for (int j = 0; j < 3; j++) v[j] = (j + 1) * step < n ? f(lo + (j + 1) * step) : ~0ull;
-        const int c = (v[0] <= goal) + (v[1] <= goal) + (v[2] <= goal);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+            if (v[j] <= goal) {
+                c++;
+                at_lo = v[j];
+            }
         lo += c * step;
         n = min(step, n - c * step);
     }
@@ -974,18 +980,13 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     const bool greedy = st.greedy;
     const uint64_t goal = greedy ? 0ull : goal_of(u, total);
     int lo;
-    uint64_t rest;
-    if (staged) {
-        lo = last_not_above(g.chunks, goal, [&](int i) { return sums[i]; });
-        rest = goal - sums[lo];
-    } else {
-        lo = last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; });
-        rest = goal - chunk_sum[lo];
-    }
+    uint64_t before, run;
+    if (staged) lo = last_not_above(g.chunks, goal, [&](int i) { return sums[i]; }, before);
+    else lo = last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; }, before);
+    const uint64_t rest = goal - before;
     const ChunkView<CUT> v(g, st, r, lo);
-    const int seg = last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); });
-    uint64_t run = v.sum_before(seg);
-    uint32_t rank = (CUT && v.thr) ? v.seg_ties[seg] : 0u;
+    const int seg = last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); }, run);
+    uint32_t rank = (CUT && v.cut) ? v.seg_ties[seg] : 0u;   // (where nothing is cut, every rank is below `left`)
     const char *row = row_base<DT>(a, r);
     const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
     const Scale s = st.scale;
