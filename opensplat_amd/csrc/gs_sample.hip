@@ -229,18 +229,32 @@ static __device__ __forceinline__ uint64_t fixed(double w, double unit) {
     return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) - 0x4330000000000000ull;
 }
 
+// Inclusive sum over the wave's lanes without LDS: shifts by 1, 2, 4, 8 inside rows of 16, then each row's last lane into
+// the next row, then lane 31 into the upper half.
+template <int CTRL, int ROWS>
+static __device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+}
+template <int CTRL, int ROWS>
+static __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+    return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
+}
+template <typename T>
+static __device__ __forceinline__ T wave_scan(T v) {
+    v += from_lane<0x111, 0xF>(v);
+    v += from_lane<0x112, 0xF>(v);
+    v += from_lane<0x114, 0xF>(v);
+    v += from_lane<0x118, 0xF>(v);
+    v += from_lane<0x142, 0xA>(v);
+    v += from_lane<0x143, 0xC>(v);
+    return v;
+}
+
 // Exclusive scan over the workgroup in thread order, THREADS a multiple of 64; `total` gets the sum.
 template <int THREADS, typename T>
 static __device__ __forceinline__ T block_scan(T v, T *wave_sums /* LDS [THREADS / 64] */, T &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T s = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(s, off, 64);
-        if (lane >= off) s += o;
-    }
-    T before = __shfl_up(s, 1, 64);
-    if (lane == 0) before = T(0);
+    const T s = wave_scan(v), before = s - v;
     if constexpr (THREADS == 64) {
         total = __shfl(s, 63, 64);
         return before;
@@ -275,21 +289,22 @@ static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goa
     uint64_t total;
     uint64_t run = above + block_scan<THREADS>(mine, wave_sums, total);
     const double need = goal_is_share ? share * (double)total : goal;
-    if (tid == 0) *out = {kBins, 0, total};
+    if (tid == 0) out->digit = kBins;
     __syncthreads();
     // the first thread whose part crosses: its start is below the goal, its end is not
     if ((double)run < need && (double)(run + mine) >= need && mine > 0) {
         for (int j = 0; j < per; j++) {
             const uint64_t b = bin(high - j);
             if (b > 0 && (double)(run + b) >= need) {
-                *out = {(uint32_t)(high - j), run, total};
+                out->digit = (uint32_t)(high - j);
+                out->above = run;
                 break;
             }
             run += b;
         }
     }
     __syncthreads();
-    const Picked p = *out;
+    const Picked p = {out->digit, out->above, total};
     __syncthreads();
     return p;
 }
@@ -315,9 +330,12 @@ constexpr int kEach = 8;                       // entries per thread
 template <int DT, bool OPACITY, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    __shared__ uint64_t kept_w[kEach][THREADS + 1];   // weight of entry 8 t + e at [e][t]; 0: not kept
+    // In turn: the masses of a digit, in copies by lane (neighbouring values share a first digit, a wave's atomics would hit
+    // few words); the weights of entry 8 t + e at [e][t], 0 if it is not kept.
+    constexpr int kPitch = THREADS + 1, kRowCopies = THREADS >= 1024 ? 4 : 1;
+    __shared__ uint64_t buffer[kEach * kPitch > kBins * kRowCopies ? kEach * kPitch : kBins * kRowCopies];
+    uint64_t *mass = buffer, *kept_w = buffer;
     __shared__ uint64_t run_sum[THREADS];
-    __shared__ uint64_t mass[kBins];
     __shared__ uint32_t count[kBins];
     __shared__ uint64_t waves_u[THREADS / 64];
     __shared__ uint32_t waves_i[THREADS / 64];
@@ -384,15 +402,17 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         uint64_t have = 0;
         for (int level = 0; level < kUsedLevels<DT>; level++) {
             for (int b = tid; b < kBins; b += THREADS) {
-                mass[b] = 0;
+#pragma unroll
+                for (int c = 0; c < kRowCopies; c++) mass[c * kBins + b] = 0;
                 count[b] = 0;
             }
             __syncthreads();
+            uint64_t *copy = mass + (tid & (kRowCopies - 1)) * kBins;
 #pragma unroll
             for (int e = 0; e < kEach; e++)
                 if (key[e] > kthr && agrees(key[e], f.found, level)) {
                     const uint32_t d = digit_of(key[e], level);
-                    atomicAdd((unsigned long long *)&mass[d], (unsigned long long)fixed(w[e], a.unit));
+                    atomicAdd((unsigned long long *)&copy[d], (unsigned long long)fixed(w[e], a.unit));
                     if (level == kUsedLevels<DT> - 1) atomicAdd(&count[d], 1u);
                 }
             __syncthreads();
@@ -402,7 +422,12 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
                 count[d] += kties;
             }
             __syncthreads();
-            const Picked p = pick_digit<THREADS>([&](int i) { return mass[i]; }, f.above, f.goal, level == 0, set.top_p,
+            const Picked p = pick_digit<THREADS>([&](int i) {
+                uint64_t m = mass[i];
+#pragma unroll
+                for (int c = 1; c < kRowCopies; c++) m += mass[c * kBins + i];
+                return m;
+            }, f.above, f.goal, level == 0, set.top_p,
                                                  waves_u, &pick);
             if (level == 0) f.goal = set.top_p * (double)p.total;
             if (p.digit == kBins) {            // (nothing weighs anything in fixed point but the first)
@@ -434,7 +459,7 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         const bool keep = key[e] > thr || (tied && rank < ties);
         rank += tied;
         const uint64_t v = (keep && w[e] >= set.min_p) ? fixed(w[e], a.unit) : 0ull;
-        kept_w[e][tid] = v;
+        kept_w[e * kPitch + tid] = v;
         sum += v;
     }
     uint64_t total;
@@ -451,7 +476,7 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         }
         uint64_t c = run_sum[lo];
         int e = -1;
-        do c += kept_w[++e][lo];
+        do c += kept_w[++e * kPitch + lo];
         while (c <= goal && e < kEach - 1);
         ids[(size_t)r * a.draws + j] = isnan(u) ? -1 : lo * kEach + e;
     }
