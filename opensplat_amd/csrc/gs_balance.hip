@@ -260,7 +260,7 @@ k_balance_grad(BalanceGrid g, int N, int nparts, const double2 *__restrict__ par
     q = block_sum_f64<kBalThreads>(q, red);
     s = block_sum_f64<kBalThreads>(s, red);
     const double m = (double)*entries;
-    const bool some = m > 0.0 && s > 0.0;
+    const bool some = m > 0.0 && s != 0.0;     // (a NaN among the opacities shows in all that depends on it)
     const double norm = some ? (double)g.tw * (double)g.th / m : 0.0, mean = some ? q / s : 0.0;
     if (blockIdx.x == 0 && threadIdx.x == 0) loss[0] = (float)(scale * (norm * mean));
     if (!v_opacity) return;

@@ -244,6 +244,7 @@ extern "C" int gs_relocate(int N, int K, int pairs, const int32_t *targets, cons
     if (N <= 0 || K < 1 || pairs < 0 || !params || !(min_opacity > 0.0f && min_opacity < 1.0f))
         return GS_ERR_INVALID_ARGUMENT;
     if (pairs == 0) return GS_OK;
+    if (pairs > 0x0fffffff) return GS_ERR_UNSUPPORTED;   // (a launch's threads, 32 bits)
     if (!targets || !sources || !workspace || ((uintptr_t)workspace & 15)) return GS_ERR_INVALID_ARGUMENT;
     const GsGaussianSet none = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     const GsGaussianSet &p = *params, &m = exp_avg ? *exp_avg : none, &v = exp_avg_sq ? *exp_avg_sq : none;

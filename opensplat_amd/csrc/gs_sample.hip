@@ -335,8 +335,10 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
     constexpr int kPitch = THREADS + 1, kRowCopies = THREADS >= 1024 ? 4 : 1;
     __shared__ uint64_t buffer[kEach * kPitch > kBins * kRowCopies ? kEach * kPitch : kBins * kRowCopies];
     uint64_t *mass = buffer, *kept_w = buffer;
-    __shared__ uint64_t run_sum[THREADS];
-    __shared__ uint32_t count[kBins];
+    // In turn: the counts of a digit, the running sums.
+    __shared__ uint64_t second[kBins / 2];
+    uint32_t *count = reinterpret_cast<uint32_t *>(second);
+    uint64_t *run_sum = second;
     __shared__ uint64_t waves_u[THREADS / 64];
     __shared__ uint32_t waves_i[THREADS / 64];
     __shared__ Picked pick;
@@ -1209,9 +1211,14 @@ extern "C" int gs_sample(int rows, int cols, const void *logits, int64_t row_str
     if (((uintptr_t)logits & (size - 1)) || ((uintptr_t)workspace & 15) || (((uintptr_t)uniforms | (uintptr_t)ids) & 3))
         return GS_ERR_INVALID_ARGUMENT;
     const SampleLayout L(rows, cols);
-    // a launch's workgroups, 31 bits
-    if ((int64_t)rows * (((int64_t)draws + kDrawThreads - 1) / kDrawThreads) > 0x7fffffffLL || (int64_t)rows * L.chunks > 0x7fffffffLL)
-        return GS_ERR_INVALID_ARGUMENT;
+    // a launch's threads, 32 bits
+    const int64_t row_threads = cols <= 64 * kEach ? 64 : (cols <= 256 * kEach ? 256 : 1024);
+    const int64_t most = L.chunks == 0 ? rows * row_threads
+                                       : (int64_t)rows * (L.chunks > kHistThreads / kChunkThreads ? (int64_t)L.chunks * kChunkThreads
+                                                                                                  : (int64_t)kHistThreads);
+    if (most > 0xffffffffLL ||
+        (L.chunks && (int64_t)rows * (((int64_t)draws + kDrawThreads - 1) / kDrawThreads) * kDrawThreads > 0xffffffffLL))
+        return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < L.total) return GS_ERR_WORKSPACE;
     SampleArgs a = {logits, row_stride, rows, cols, draws, 0.0, *cfg};
     int log_cols = 0;

@@ -148,6 +148,27 @@ def test_sample_large_row_with_many_draws():
     check_sample(dev(x), u, True, top_k=700_001, min_p=0.5)
 
 
+@pytest.mark.parametrize("opt", [dict(), dict(top_k=9_000_000, min_p=0.2), dict(top_p=0.7, temperature=0.5)])
+def test_sample_row_of_more_chunks_than_a_table_holds(opt):
+    """17 M entries: the forms for rows whose chunks' maxima and running sums do not fit beside a workgroup."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((1, 17_000_003), device="cuda", generator=g).bfloat16()
+    x[0, 5_000_000:6_000_000] = -torch.inf
+    for draws in (7, 20_000):
+        check_sample(x, torch.rand((1, draws), device="cuda", generator=g), **opt)
+
+
+@pytest.mark.parametrize("shape", [(3000, 28, 2), (700, 1500, 3), (300, 8000, 2), (300, 9000, 40)])
+def test_sample_many_rows(shape):
+    rows, cols, draws = shape
+    rng = np.random.default_rng(rows)
+    x, u = logits_of(rng, rows, cols, "f16", pad=3), dev(rng.random((rows, draws), dtype=np.float32))
+    x[::7] = -np.inf
+    p = dev((0.3 + 0.8 * rng.random(rows)).astype(np.float32))
+    k = dev(rng.integers(0, 60, rows).astype(np.int32))
+    check_sample(x, u, top_p=p, top_k=k, temperature=0.9)
+
+
 def test_sample_rows_beyond_32_bit_offsets():
     """The last rows start more than 2^31 elements behind the first."""
     rows, cols, stride = 5, 1000, 600_000_000
@@ -263,6 +284,11 @@ def test_tile_balance_of_nothing():
     p[:, 5] = 0
     loss, _, v = cabi.tile_balance(64, 64, dev(p), dev(bins))
     assert float(loss[0]) == 0 and (v == 0).all()
+    # a NaN opacity is not swallowed
+    p[3, 5] = np.nan
+    covered = (p[3, 7].view(np.uint32) >> 16) > 0
+    loss, _, v = cabi.tile_balance(64, 64, dev(p), dev(bins))
+    assert bool(torch.isnan(loss[0])) == covered
 
 
 def test_tile_balance_of_a_binned_frame():

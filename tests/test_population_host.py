@@ -26,9 +26,16 @@ def sample(rows=2, cols=5, logits=ONE, stride=5, draws=3, u=ONE, ids=ONE, ws=ONE
                                 dict(top_p=float("nan")), dict(min_p=1.5), dict(min_p=float("nan")),
                                 dict(logits=C.c_void_p(66)), dict(logits=C.c_void_p(65), dtype=1),
                                 dict(ws=C.c_void_p(72)), dict(ids=C.c_void_p(66)), dict(u=C.c_void_p(66)),
-                                dict(rows=1 << 30, draws=1 << 30)])
+                                ])
 def test_sample_refuses(kw):
     assert sample(**kw) == INVALID
+
+
+def test_sample_limits():
+    """More threads than a launch can have."""
+    assert sample(rows=1 << 27) == UNSUPPORTED and sample(rows=1 << 23, cols=8000, stride=8000) == UNSUPPORTED
+    assert sample(rows=1 << 20, cols=1 << 20, stride=1 << 20) == UNSUPPORTED
+    assert sample(rows=1 << 12, cols=9000, stride=9000, draws=1 << 21) == UNSUPPORTED
 
 
 def test_sample_workspace_and_empty_calls():
@@ -77,6 +84,7 @@ def test_relocate_workspace_and_empty_calls():
     need = cabi.lib().gs_relocate_workspace_bytes(9, 2)
     assert need > 0 and relocate(size=need - 1) == WORKSPACE
     assert relocate(pairs=0) == 0
+    assert relocate(pairs=1 << 29) == UNSUPPORTED
 
 
 def test_host_tensors_are_refused():
