@@ -514,7 +514,8 @@ struct LongArgs {
     uint64_t *chunk_sum;                       // [rows][chunks]: sums, then running sums
     uint32_t *chunk_ties;                      // [rows][chunks]: ties, then running ties
     uint64_t *seg_sum;                         // [rows][chunks][kChunkSegs] running sums inside the chunk
-    uint32_t *seg_ties;
+    uint64_t *mid_sum, *top_sum;               // every 8th and every 64th of them again, for the draws' first steps
+    uint32_t *seg_ties;                        // [rows][chunks][kChunkSegs]
     int chunks;
     bool with_k, with_p;                       // launches that look for a threshold
 };
@@ -659,6 +660,12 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
     __shared__ Picked pick;
     const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
     LongRow &st = g.rows[r];
+    // the first entries are under way while the digit before this one is picked
+    const char *row = row_base<DT>(a, r);
+    const int64_t n = a.cols, step = (int64_t)kHistThreads * kVec<DT>, first = (int64_t)part * kBatch * step;
+    uint32_t k[kBatch][kVec<DT>];
+#pragma unroll
+    for (int q = 0; q < kBatch; q++) keys_at<DT>(row, first + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
     uint32_t k_thr = 0, k_ties = 0;
     Search f;
     if constexpr (MASS) {
@@ -694,8 +701,6 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
         count[b] = 0;
     }
     __syncthreads();
-    const char *row = row_base<DT>(a, r);
-    const int64_t n = a.cols, step = (int64_t)kHistThreads * kVec<DT>;
     const int lane = tid & 63, copy = lane & (copies - 1);
     auto add = [&](uint32_t key) {
         const uint32_t d = digit_of(key, level);
@@ -709,11 +714,11 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
     };
     uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? kBins : 0)) + (tid >> 6) * 128;
     int waiting = 0;
-    for (int64_t i0 = (int64_t)part * kBatch * step + (int64_t)tid * kVec<DT>; i0 - (int64_t)tid * kVec<DT> < n;
-         i0 += (int64_t)parts * kBatch * step) {
-        uint32_t k[kBatch][kVec<DT>];
+    for (int64_t i0 = first; i0 < n; i0 += (int64_t)parts * kBatch * step) {
+        if (i0 != first) {
 #pragma unroll
-        for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + q * step, n, k[q]);
+            for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
+        }
 #pragma unroll
         for (int q = 0; q < kBatch; q++)
 #pragma unroll
@@ -861,6 +866,8 @@ k_long_sums(SampleArgs a, LongArgs g) {
     uint64_t total;
     const uint64_t before = block_scan<kChunkThreads>(sum[0] + sum[1], waves_u, total);
     *reinterpret_cast<ulonglong2 *>(g.seg_sum + seg) = make_ulonglong2(before, before + sum[0]);
+    if ((tid & 3) == 0) g.mid_sum[at * (kChunkSegs / 8) + (tid >> 2)] = before;
+    if ((tid & 31) == 0) g.top_sum[at * (kChunkSegs / 64) + (tid >> 5)] = before;
     if (tid == 0) g.chunk_sum[at] = total;
     if constexpr (CUT) {
         if (thr) {
@@ -907,40 +914,22 @@ k_long_scan(LongArgs g) {
     if (tid == 0) st.total = ok ? base : 0ull;
 }
 
-// The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not exceed `goal`, and that value; four-fold steps,
-// whose three loads are under way together.
-template <typename F>
-static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f, uint64_t &at_lo) {
-    int lo = 0;
-    at_lo = 0;
-    while (n > 1) {
-        const int step = (n + 3) >> 2;
-        uint64_t v[3];
-#pragma unroll
-        for (int j = 0; j < 3; j++) v[j] = (j + 1) * step < n ? f(lo + (j + 1) * step) : ~0ull;
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < 3; j++)
-            if (v[j] <= goal) {
-                c++;
-                at_lo = v[j];
-            }
-        lo += c * step;
-        n = min(step, n - c * step);
-    }
-    return lo;
+// A draw is made by LANES neighbouring lanes.  The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not
+// exceed `goal`, LANES values at a time; each of the lanes gets it.
+template <int LANES>
+static __device__ __forceinline__ uint64_t group_ballot(bool b) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(b) >> (threadIdx.x & 63 & ~(LANES - 1));
+    return LANES == 64 ? m : m & ((1ull << (LANES & 63)) - 1ull);
 }
-// The same by a wave, 64 values at a time; every lane gets it.
-template <typename F>
-static __device__ __forceinline__ int wave_last_not_above(int n, uint64_t goal, F f) {
-    const int lane = threadIdx.x & 63;
+template <int LANES, typename F>
+static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f) {
+    const int lane = threadIdx.x & (LANES - 1);
     int lo = 0;
-    while (n > 1) {
-        const int step = (n + 63) / 64, at = lane * step;
-        const bool below = at < n && f(lo + at) <= goal;
-        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(below)) - 1;   // (f(lo) <= goal)
+    while (n > 1) {                            // (n is the same in every lane of the wave)
+        const int step = (n + LANES - 1) / LANES, at = lane * step;
+        const int c = __builtin_popcountll(group_ballot<LANES>(at < n && f(lo + at, step) <= goal)) - 1;   // (f(lo) <= goal)
         lo += c * step;
-        n = min(step, n - c * step);
+        n = step;
     }
     return lo;
 }
@@ -949,7 +938,7 @@ static __device__ __forceinline__ int wave_last_not_above(int n, uint64_t goal, 
 // ones behind the `left` first are taken off.
 template <bool CUT>
 struct ChunkView {
-    const uint64_t *seg_sum;
+    const uint64_t *seg_sum, *mid_sum, *top_sum;
     const uint32_t *seg_ties;
     uint64_t tie_weight;
     uint32_t thr, left;
@@ -957,6 +946,8 @@ struct ChunkView {
     __device__ ChunkView(const LongArgs &g, const LongRow &st, int r, int c) {
         const size_t chunk = (size_t)r * g.chunks + c;
         seg_sum = g.seg_sum + chunk * kChunkSegs;
+        mid_sum = g.mid_sum + chunk * (kChunkSegs / 8);
+        top_sum = g.top_sum + chunk * (kChunkSegs / 64);
         seg_ties = g.seg_ties + chunk * kChunkSegs;
         tie_weight = 0;
         thr = CUT ? st.thr : 0u;
@@ -969,8 +960,9 @@ struct ChunkView {
             cut = c + 1 == g.chunks || g.chunk_ties[chunk + 1] - before > left;
         }
     }
-    __device__ uint64_t sum_before(int i) const {
-        uint64_t v = seg_sum[i];
+    // (i a multiple of `step`: neighbours of a step lie side by side, a draw touches a line per step)
+    __device__ uint64_t sum_before(int i, int step) const {
+        uint64_t v = step == 64 ? top_sum[i >> 6] : (step == 8 ? mid_sum[i >> 3] : seg_sum[i]);
         if (CUT && cut) {
             const uint32_t t = seg_ties[i];
             if (t > left) v -= tie_weight * (t - left);
@@ -979,114 +971,56 @@ struct ChunkView {
     }
 };
 
-// Many draws: one thread each.  The last chunk, then the last 8 entries, whose running sum does not exceed the goal, then
-// entry by entry.  (Integer sums: what is found there holds a weight.)  A workgroup's draws are of one row; its chunks'
-// running sums are searched in LDS where they fit.
-constexpr int kDrawThreads = 256;
-constexpr int kDrawChunks = 4096;
-template <int DT, bool OPACITY, bool CUT>
-__global__ void __launch_bounds__(kDrawThreads)
+// A draw: the last chunk, then the last 8 entries, whose running sum does not exceed the goal, then these side by side.
+// (Integer sums: what is found there holds a weight.)  Bound by the latency of six or seven dependent loads, which the
+// other draws' hide: eight lanes a draw make 31 000 waves of 250 000 draws, where a thread a draw left four to a SIMD.
+// A workgroup's draws are of one row, so that what a row has in common stays in scalar registers.
+template <int LANES>
+constexpr int kDrawThreads = LANES == 64 ? 64 : 256;
+template <int DT, bool OPACITY, bool CUT, int LANES>
+__global__ void __launch_bounds__(kDrawThreads<LANES>)
 k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    extern __shared__ uint64_t sums[];
-    const int r = blockIdx.x / blocks, j = (blockIdx.x - r * blocks) * kDrawThreads + threadIdx.x;
-    const LongRow &st = g.rows[r];
-    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-    const bool staged = g.chunks <= kDrawChunks;
-    if (staged) {
-        for (int c = threadIdx.x; c < g.chunks; c += kDrawThreads) sums[c] = chunk_sum[c];
-        __syncthreads();
-    }
-    if (j >= a.draws) return;
-    const size_t at = (size_t)r * a.draws + j;
-    const uint64_t total = st.total;
-    const float u = uniforms[at];
-    if (total == 0 || isnan(u)) {
-        ids[at] = -1;
-        return;
-    }
-    const bool greedy = st.greedy;
-    const uint64_t goal = greedy ? 0ull : goal_of(u, total);
-    int lo;
-    uint64_t before, run;
-    if (staged) lo = last_not_above(g.chunks, goal, [&](int i) { return sums[i]; }, before);
-    else lo = last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; }, before);
-    const uint64_t rest = goal - before;
-    const ChunkView<CUT> v(g, st, r, lo);
-    const int seg = last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); }, run);
-    uint32_t rank = (CUT && v.cut) ? v.seg_ties[seg] : 0u;   // (where nothing is cut, every rank is below `left`)
-    const char *row = row_base<DT>(a, r);
-    const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
-    const Scale s = st.scale;
-    const double min_p = st.min_p;
-    uint32_t key[kSeg];
-#pragma unroll
-    for (int q = 0; q < kSeg / kVec<DT>; q++) {
-        uint32_t k[kVec<DT>];
-        keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
-#pragma unroll
-        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
-    }
-    int id = -1;
-#pragma unroll
-    for (int e = 0; e < kSeg; e++) {
-        const bool tied = CUT && v.thr != 0 && key[e] == v.thr;
-        const bool keep = key[e] > v.thr || (tied && rank < v.left);
-        rank += tied;
-        if (id >= 0 || !keep || (greedy && key[e] != s.top)) continue;
-        const double w = weight<DT, OPACITY>(key[e], s);
-        if (w >= min_p) run += fixed(w, a.unit);
-        if (run > rest) id = e;
-    }
-    ids[at] = id < 0 ? -1 : (int32_t)(i0 + id);
-}
-
-// Few draws: a wave each, 64 running sums and then the 8 entries side by side; four dependent loads instead of twenty.
-template <int DT, bool OPACITY, bool CUT>
-__global__ void __launch_bounds__(64)
-k_long_draw_wave(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    const int at = blockIdx.x, r = at / a.draws, lane = threadIdx.x;
+    const int r = blockIdx.x / blocks, lane = threadIdx.x & (LANES - 1);
+    const int mine = (blockIdx.x - r * blocks) * (kDrawThreads<LANES> / LANES) + threadIdx.x / LANES;
+    // (lanes without a draw repeat the last: a wave's steps are in common)
+    const size_t at = (size_t)r * a.draws + min(mine, a.draws - 1);
     const LongRow &st = g.rows[r];
     const uint64_t total = st.total;
     const float u = uniforms[at];
-    if (total == 0 || isnan(u)) {
-        if (lane == 0) ids[at] = -1;
-        return;
-    }
-    const bool greedy = st.greedy;
-    const uint64_t goal = greedy ? 0ull : goal_of(u, total);
+    const bool none = total == 0 || isnan(u), greedy = st.greedy;
+    const uint64_t goal = (greedy || none) ? 0ull : goal_of(u, total);
     const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-    const int lo = wave_last_not_above(g.chunks, goal, [&](int i) { return chunk_sum[i]; });
+    const int lo = last_not_above<LANES>(g.chunks, goal, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; });
     const uint64_t rest = goal - chunk_sum[lo];
     const ChunkView<CUT> v(g, st, r, lo);
-    const int seg = wave_last_not_above(kChunkSegs, rest, [&](int i) { return v.sum_before(i); });
-    const uint64_t before = v.sum_before(seg);
-    const uint32_t ties_before = (CUT && v.thr) ? v.seg_ties[seg] : 0u;
+    const int seg = last_not_above<LANES>(kChunkSegs, rest, [&](int i, int step) { return v.sum_before(i, step); });
+    const uint64_t before = v.sum_before(seg, 1);
     const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
     uint32_t key = 0;
     if (lane < kSeg && i0 + lane < a.cols) key = key_at<DT>(row_base<DT>(a, r), i0 + lane);
     const bool tied = CUT && v.thr != 0 && key == v.thr;
-    const uint32_t rank =
-        ties_before + __builtin_popcountll(__builtin_amdgcn_ballot_w64(tied) & ((1ull << lane) - 1ull));
-    uint64_t mine = 0;
+    uint32_t rank = 0;                         // (where nothing is cut, every rank is below `left`)
+    if (CUT && v.cut) rank = v.seg_ties[seg];
+    rank += __builtin_popcountll(group_ballot<LANES>(tied) & ((1ull << lane) - 1ull));
+    uint64_t run = 0;
     if ((key > v.thr || (tied && rank < v.left)) && (!greedy || key == st.scale.top)) {
         const double w = weight<DT, OPACITY>(key, st.scale);
-        if (w >= st.min_p) mine = fixed(w, a.unit);
+        if (w >= st.min_p) run = fixed(w, a.unit);
     }
-    uint64_t run = mine;
 #pragma unroll
     for (int off = 1; off < kSeg; off <<= 1) {
         const uint64_t o = __shfl_up(run, off, 64);
         if (lane >= off) run += o;
     }
-    const uint64_t over = __builtin_amdgcn_ballot_w64(lane < kSeg && before + run > rest);
-    if (lane == 0) ids[at] = over ? (int32_t)(i0 + __builtin_ctzll(over)) : -1;
+    const uint64_t over = group_ballot<LANES>(lane < kSeg && before + run > rest);
+    if (lane == 0 && mine < a.draws) ids[at] = (none || over == 0) ? -1 : (int32_t)(i0 + __builtin_ctzll(over));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 constexpr int kRowLimit = 8192;                // longest row of the one-workgroup form
 
 struct SampleLayout {
-    size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, seg_ties, total;
+    size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, mid_sum, top_sum, seg_ties, total;
     int chunks;
     SampleLayout(int n_rows, int cols) {
         size_t o = 0;
@@ -1101,6 +1035,8 @@ struct SampleLayout {
         chunk_sum = take(n * 8);
         chunk_ties = take(n * 4);
         seg_sum = take(n * kChunkSegs * 8);
+        mid_sum = take(n * kChunkSegs);
+        top_sum = take(n * kChunkSegs / 8);
         seg_ties = take(n * kChunkSegs * 4);
         total = o > 0 ? o : 256;
     }
@@ -1124,7 +1060,8 @@ static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids,
 // would grow with the square of the row.
 constexpr int kOwnMaxChunks = 4096;
 
-constexpr int64_t kWaveDraws = 8192;
+// Up to this many draws a wave each: four dependent loads instead of six.
+constexpr int64_t kWaveDraws = 2048;
 
 template <int DT, bool OPACITY, bool CUT>
 static int launch_long(const SampleArgs &a, const LongArgs &g, const float *uniforms, int32_t *ids, hipStream_t s) {
@@ -1163,13 +1100,13 @@ static int launch_long(const SampleArgs &a, const LongArgs &g, const float *unif
     GS_LAUNCH_CHECK();
     GS_LAUNCH((k_long_scan<CUT>), rows, dim3(kHistThreads), 0, s, g);
     GS_LAUNCH_CHECK();
-    // A wave per draw while the waves are all resident; at 64 rows of 131072 and one draw each 5 us against 10.
     if ((int64_t)a.rows * a.draws <= kWaveDraws) {
-        GS_LAUNCH((k_long_draw_wave<DT, OPACITY, CUT>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g, uniforms, ids);
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 64>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g, a.draws,
+                  uniforms, ids);
     } else {
-        const int blocks = (a.draws + kDrawThreads - 1) / kDrawThreads;
-        const size_t lds = g.chunks <= kDrawChunks ? (size_t)g.chunks * 8 : 0;
-        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT>), dim3((unsigned)(blocks * a.rows)), dim3(kDrawThreads), lds, s, a, g, blocks, uniforms, ids);
+        const int blocks = (int)(((int64_t)a.draws + 31) / 32);
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 8>), dim3((unsigned)((int64_t)blocks * a.rows)), dim3(256), 0, s, a, g, blocks,
+                  uniforms, ids);
     }
     GS_LAUNCH_CHECK();
     return GS_OK;
@@ -1183,7 +1120,8 @@ static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *id
     const bool with_k = c.top_k_rows || c.top_k > 0, with_p = c.top_p_rows || c.top_p < 1.0f;
     const LongArgs g = {(LongRow *)(ws + L.rows), (uint32_t *)(ws + L.k_count), (uint64_t *)(ws + L.p_mass),
                         (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
-                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint32_t *)(ws + L.seg_ties),
+                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint64_t *)(ws + L.mid_sum),
+                        (uint64_t *)(ws + L.top_sum), (uint32_t *)(ws + L.seg_ties),
                         L.chunks, with_k, with_p};
     return with_k || with_p ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
                             : launch_long<DT, OPACITY, false>(a, g, uniforms, ids, s);
@@ -1217,7 +1155,7 @@ extern "C" int gs_sample(int rows, int cols, const void *logits, int64_t row_str
                                        : (int64_t)rows * (L.chunks > kHistThreads / kChunkThreads ? (int64_t)L.chunks * kChunkThreads
                                                                                                   : (int64_t)kHistThreads);
     if (most > 0xffffffffLL ||
-        (L.chunks && (int64_t)rows * (((int64_t)draws + kDrawThreads - 1) / kDrawThreads) * kDrawThreads > 0xffffffffLL))
+        (L.chunks && (int64_t)rows * (((int64_t)draws + 31) / 32) > 0xffffffffLL / 256))
         return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < L.total) return GS_ERR_WORKSPACE;
     SampleArgs a = {logits, row_stride, rows, cols, draws, 0.0, *cfg};
