@@ -493,6 +493,7 @@ constexpr int kLevels = 3;
 constexpr int kHistThreads = 1024;
 constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
 constexpr int kCopies = 4;
+constexpr int kQueue = 640;                    // keys a wave can have waiting
 
 // A row's state between the launches.  A launch reads what earlier ones wrote and writes other fields.
 struct LongRow {
@@ -712,7 +713,8 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
             atomicAdd(&count[d], 1u);
         }
     };
-    uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? kBins : 0)) + (tid >> 6) * 128;
+    static_assert(63 + 64 * 8 <= kQueue && kQueue * (kHistThreads / 64) * 4 <= kBins * (kCopies - 1) * 8, "a load's keys and a rest");
+    uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? kBins : 0)) + (tid >> 6) * kQueue;
     int waiting = 0;
     for (int64_t i0 = first; i0 < n; i0 += (int64_t)parts * kBatch * step) {
         if (i0 != first) {
@@ -720,25 +722,30 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
             for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
         }
 #pragma unroll
-        for (int q = 0; q < kBatch; q++)
+        for (int q = 0; q < kBatch; q++) {
+            uint32_t in = 0;
 #pragma unroll
-            for (int e = 0; e < kVec<DT>; e++) {
-                const bool in = k[q][e] > k_thr && agrees(k[q][e], f.found, level);
-                if (!queued) {
-                    if (in) add(k[q][e]);
-                    continue;
-                }
-                const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-                if (m == 0) continue;
-                if (in) wave_queue[waiting + __builtin_popcountll(m & ((1ull << lane) - 1ull))] = k[q][e];
-                waiting += __builtin_popcountll(m);
-                if (waiting >= 64) {
-                    waiting -= 64;
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    add(wave_queue[waiting + lane]);
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                }
+            for (int e = 0; e < kVec<DT>; e++)
+                in |= (k[q][e] > k_thr && agrees(k[q][e], f.found, level)) ? 1u << e : 0u;
+            if (!queued) {
+#pragma unroll
+                for (int e = 0; e < kVec<DT>; e++)
+                    if ((in >> e) & 1u) add(k[q][e]);
+                continue;
             }
+            const uint32_t mine = __builtin_popcount(in), upto = wave_scan(mine);
+            int at = waiting + (int)(upto - mine);
+#pragma unroll
+            for (int e = 0; e < kVec<DT>; e++)
+                if ((in >> e) & 1u) wave_queue[at++] = k[q][e];
+            waiting += __builtin_amdgcn_readlane((int)upto, 63);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            while (waiting >= 64) {
+                waiting -= 64;
+                add(wave_queue[waiting + lane]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
     }
     if (queued) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
