@@ -14,7 +14,9 @@
 // Larger frames: k_balance_rows and k_balance_cols leave the table in memory.
 //
 // Bound by the records' lines: 12 of a record's 48 bytes are used and no line is without some, 240 MB at 5 M Gaussians.
-// The second launch reads the 12 bytes kept (60 MB) instead of the records again.
+// The second launch reads the 12 bytes kept (60 MB) instead of the records again.  Measured: 1 M Gaussians at 1080p 19 + 6
+// us, 5 M at 4K 74 + 14 us (4.1 TB/s in the first launch, a large copy reaches 4.9; 5 us of it before the table is made).
+// With the table from memory and the records read twice it was 48 and 164 us.
 #include <math.h>
 
 #include "gs_device.h"

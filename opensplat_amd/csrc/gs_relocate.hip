@@ -20,7 +20,8 @@
 // stay as they are.
 //
 // Bound by scattered lines: a row of 59 floats lies in six places (some nine 64-byte lines), written for the copy in
-// parameters and moments, and in the moments for the source.
+// parameters and moments, and in the moments for the source: some 56 lines a pair.  Measured: 300 pairs 5.6 + 6.7 us, 50 000
+// of a million Gaussians 19 + 39 us from the caches, 100 us from memory.
 #include <math.h>
 
 #include "gs_device.h"
