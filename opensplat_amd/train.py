@@ -252,16 +252,18 @@ class Trainer:
                 self._g_stream = torch.cuda.Stream()
 
     def _balance_buffers(self, W, H):
-        """-> (loss [1], entries per tile, the opacities' gradient) and a workspace, for _balance."""
+        """-> (loss [1], entries per tile) and a workspace, for _balance."""
         dev = self.dev
         tiles = ((W + cabi.GS_TILE - 1) // cabi.GS_TILE) * ((H + cabi.GS_TILE - 1) // cabi.GS_TILE)
-        return (torch.empty(1, device=dev), torch.empty(tiles, device=dev, dtype=torch.int32), self.grads.v_opacity), \
+        return (torch.empty(1, device=dev), torch.empty(tiles, device=dev, dtype=torch.int32)), \
             torch.empty(cabi.lib().gs_tile_balance_workspace_bytes(W, H, self.N), device=dev, dtype=torch.uint8)
 
     def _balance(self, W, H, b, scale, out, workspace):
         """The balance loss of the frame's lists, its gradient added to the opacities' (behind gaussian_backward)."""
+        # (a refinement replaces the gradient buffer, of the same size perhaps: never kept with the frame's buffers)
         cabi.tile_balance(W, H, b.packed, b.tile_bins, scale * self.balance_weight,
-                          cabi.GS_FLAG_LOGIT_OPACITY | cabi.GS_FLAG_ACCUMULATE_GRADS, out=out, workspace=workspace)
+                          cabi.GS_FLAG_LOGIT_OPACITY | cabi.GS_FLAG_ACCUMULATE_GRADS,
+                          out=(*out, self.grads.v_opacity), workspace=workspace)
 
     def render(self, cam: dict, background, degrees_to_use: int):
         """Model::forward (model.cpp:83-225) for one camera -> clamped rgb [H, W, 3]."""

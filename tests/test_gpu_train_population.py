@@ -143,6 +143,20 @@ def test_balance_of_a_camera_batch():
     assert ((a.double() - want - sum(parts)).abs() <= 8 * 2.0 ** -24 * size + 2.0 ** -20 * want.abs().max()).all()
 
 
+def test_balance_reaches_a_replaced_gradient_buffer():
+    """A refinement that leaves the set's size as it was still replaces the gradient buffer."""
+    from opensplat_amd import dist
+
+    T, cams, gts, bg = setup(balance_weight=0.3, deterministic=True)
+    T.train_step_batch(cams, gts, bg, 1, step_optimizer=False)
+    want = T.grads.v_opacity.clone()
+    T.grads = dist.GradBuffer(T.N, T.K, T.dev)
+    T._shape = None
+    T.train_step_batch(cams, gts, bg, 1, step_optimizer=False)
+    torch.cuda.synchronize()
+    assert torch.equal(T.grads.v_opacity, want)
+
+
 def test_refused_arguments():
     for kw in (dict(strategy="other"), dict(min_opacity=0.0), dict(source_temperature=0.0), dict(source_top_p=0.0),
                dict(strategy="relocate", reference_alpha_reset=True)):
