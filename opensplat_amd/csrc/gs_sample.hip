@@ -212,6 +212,7 @@ static __device__ __forceinline__ double weight(uint32_t key, const Scale &s) {
 }
 // ---- digits of a threshold ----------------------------------------------------------------------------------------
 constexpr int kBins = 2048;
+constexpr int kLevels = 3;
 template <int DT>
 constexpr int kUsedLevels = DT == kF32 ? 3 : 2;   // a 16-bit type's key ends within the second digit
 static __device__ __forceinline__ int digit_shift(int level) { return level == 0 ? 21 : (level == 1 ? 10 : 0); }
@@ -279,8 +280,9 @@ static __device__ __forceinline__ T block_scan(T v, T *wave_sums /* LDS [THREADS
     return base + before;
 }
 
-// The digit in which the running total, from the largest digit down, reaches the goal.  `bin(i)`: count or mass of digit
-// i.  Every thread of the workgroup gets the digit and what lies above it; called with the histogram complete.
+// The digit in which the running total, from the largest digit down, reaches the goal (kBins: none does).  `bin(i)`: count
+// or mass of digit i.  Every thread of the workgroup gets the digit and what lies above it; called with the histogram
+// complete, each time with a place `out` of its own.
 struct Picked {
     uint32_t digit;
     uint64_t above, total;
@@ -290,15 +292,14 @@ static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goa
                                     uint64_t *wave_sums, Picked *out /* LDS */) {
     constexpr int per = kBins / THREADS < 1 ? 1 : kBins / THREADS;
     const int tid = threadIdx.x, high = kBins - 1 - tid * per;
+    if (tid == 0) out->digit = kBins;          // (the scan's barriers stand between this and the writer below)
     uint64_t mine = 0;
 #pragma unroll 4
     for (int j = 0; j < per; j++) mine += bin(high - j);
     uint64_t total;
     uint64_t run = above + block_scan<THREADS>(mine, wave_sums, total);
     const double need = goal_is_share ? share * (double)total : goal;
-    if (tid == 0) out->digit = kBins;
-    __syncthreads();
-    // the first thread whose part crosses: its start is below the goal, its end is not
+    // the one thread whose part crosses: its start is below the goal, its end is not
     if ((double)run < need && (double)(run + mine) >= need && mine > 0) {
         for (int j = 0; j < per; j++) {
             const uint64_t b = bin(high - j);
@@ -311,9 +312,7 @@ static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goa
         }
     }
     __syncthreads();
-    const Picked p = {out->digit, out->above, total};
-    __syncthreads();
-    return p;
+    return {out->digit, out->above, total};
 }
 
 static __device__ __forceinline__ uint32_t ties_for(uint64_t above, double goal, double tie_weight, double unit,
@@ -337,18 +336,20 @@ constexpr int kEach = 8;                       // entries per thread
 template <int DT, bool OPACITY, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    // In turn: the masses of a digit, in copies by lane (neighbouring values share a first digit, a wave's atomics would hit
-    // few words); the weights of entry 8 t + e at [e][t], 0 if it is not kept.
+    // Histograms.  1024 threads: one for every digit, emptied together, which saves two barriers of sixteen waves a digit;
+    // the first digit's masses in copies by lane (neighbouring values share it, a wave's atomics would hit few words).
+    // Fewer threads: one for all, so that many short rows share a compute unit.  The first words also hold, in turn, the
+    // weights of entry 8 t + e at [e][t], 0 if it is not kept; the counts' the running sums.
     constexpr int kPitch = THREADS + 1, kRowCopies = THREADS >= 1024 ? 4 : 1;
-    __shared__ uint64_t buffer[kEach * kPitch > kBins * kRowCopies ? kEach * kPitch : kBins * kRowCopies];
-    uint64_t *mass = buffer, *kept_w = buffer;
-    // In turn: the counts of a digit, the running sums.
-    __shared__ uint64_t second[kBins / 2];
-    uint32_t *count = reinterpret_cast<uint32_t *>(second);
-    uint64_t *run_sum = second;
+    constexpr bool kSplit = THREADS >= 1024;
+    constexpr int kFirst = kEach * kPitch > kBins * kRowCopies ? kEach * kPitch : kBins * kRowCopies;
+    __shared__ uint64_t masses[kFirst + (kSplit ? (kLevels - 1) * kBins : 0)];
+    __shared__ uint64_t counts_or_sums[(kSplit ? kLevels + 1 : 1) * kBins / 2];
+    uint32_t *counts = reinterpret_cast<uint32_t *>(counts_or_sums);
+    uint64_t *kept_w = masses, *run_sum = counts_or_sums;
     __shared__ uint64_t waves_u[THREADS / 64];
     __shared__ uint32_t waves_i[THREADS / 64];
-    __shared__ Picked pick;
+    __shared__ Picked picks[2 * kLevels];
     const int r = blockIdx.x, tid = threadIdx.x, n = a.cols;
     const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
     const RowSettings set = row_settings(a, r);
@@ -383,17 +384,30 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         if (key[e] != 0 && (!set.greedy || key[e] == mx)) w[e] = weight<DT, OPACITY>(key[e], s);
     }
     uint32_t thr = 0, ties = 0;
-    if (!set.greedy && set.top_k > 0) {
+    const bool with_k = !set.greedy && set.top_k > 0, with_p = !set.greedy && set.top_p < 1.0;
+    if (kSplit && (with_k || with_p)) {
+        if (with_p)
+            for (int b = tid; b < kBins * kRowCopies; b += THREADS) masses[b] = 0;
+        if (with_p)
+            for (int b = tid; b < (kLevels - 1) * kBins; b += THREADS) masses[kFirst + b] = 0;
+        for (int b = tid; b < (kLevels + 1) * kBins; b += THREADS) counts[b] = 0;
+        __syncthreads();
+    }
+    if (with_k) {
         Search f = {0, (double)set.top_k, 0, 0};
         for (int level = 0; level < kUsedLevels<DT> && !f.done; level++) {
-            for (int b = tid; b < kBins; b += THREADS) count[b] = 0;
-            __syncthreads();
+            uint32_t *count = counts + (kSplit ? level * kBins : 0);
+            if (!kSplit) {
+                __syncthreads();
+                for (int b = tid; b < kBins; b += THREADS) count[b] = 0;
+                __syncthreads();
+            }
 #pragma unroll
             for (int e = 0; e < kEach; e++)
                 if (key[e] != 0 && agrees(key[e], f.found, level)) atomicAdd(&count[digit_of(key[e], level)], 1u);
             __syncthreads();
             const Picked p = pick_digit<THREADS>([&](int i) { return (uint64_t)count[i]; }, f.above, f.goal, false, 0.0,
-                                                 waves_u, &pick);
+                                                 waves_u, &picks[level]);
             if (p.digit == kBins) f.done = 1;  // fewer candidates than k
             else f.found |= p.digit << digit_shift(level);
             f.above = p.above;
@@ -403,41 +417,41 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
             ties = (uint32_t)set.top_k - (uint32_t)f.above;
         }
     }
-    if (!set.greedy && set.top_p < 1.0) {
+    if (with_p) {
         const uint32_t kthr = thr, kties = ties;
-        double kw = 0.0;
-        if (kthr) kw = weight<DT, OPACITY>(kthr, s);
+        uint64_t tied = 0;                     // the ties that top-k left, as one
+        if (kthr) tied = (uint64_t)kties * fixed(weight<DT, OPACITY>(kthr, s), a.unit);
         Search f = {0, 0.0, 0, 0};
         uint64_t have = 0;
         for (int level = 0; level < kUsedLevels<DT>; level++) {
-            for (int b = tid; b < kBins; b += THREADS) {
-#pragma unroll
-                for (int c = 0; c < kRowCopies; c++) mass[c * kBins + b] = 0;
-                count[b] = 0;
+            uint64_t *mass = masses + (kSplit && level > 0 ? kFirst + (level - 1) * kBins : 0);
+            uint32_t *count = counts + (kSplit ? kLevels * kBins : 0);
+            const int copies = level == 0 ? kRowCopies : 1;
+            if (!kSplit) {
+                __syncthreads();
+                for (int b = tid; b < kBins; b += THREADS) {
+                    mass[b] = 0;
+                    count[b] = 0;
+                }
+                __syncthreads();
             }
-            __syncthreads();
-            uint64_t *copy = mass + (tid & (kRowCopies - 1)) * kBins;
+            uint64_t *copy = mass + (tid & (copies - 1)) * kBins;
+            const bool last = level == kUsedLevels<DT> - 1;
+            auto add = [&](uint32_t k, uint64_t w_, uint32_t n_) {
+                const uint32_t d = digit_of(k, level);
+                atomicAdd((unsigned long long *)&copy[d], (unsigned long long)w_);
+                if (last) atomicAdd(&count[d], n_);
+            };
 #pragma unroll
             for (int e = 0; e < kEach; e++)
-                if (key[e] > kthr && agrees(key[e], f.found, level)) {
-                    const uint32_t d = digit_of(key[e], level);
-                    atomicAdd((unsigned long long *)&copy[d], (unsigned long long)fixed(w[e], a.unit));
-                    if (level == kUsedLevels<DT> - 1) atomicAdd(&count[d], 1u);
-                }
-            __syncthreads();
-            if (tid == 0 && kthr && agrees(kthr, f.found, level)) {   // the ties that top-k left, as one
-                const uint32_t d = digit_of(kthr, level);
-                mass[d] += (uint64_t)kties * fixed(kw, a.unit);
-                count[d] += kties;
-            }
+                if (key[e] > kthr && agrees(key[e], f.found, level)) add(key[e], fixed(w[e], a.unit), 1u);
+            if (tid == 0 && kthr && agrees(kthr, f.found, level)) add(kthr, tied, kties);
             __syncthreads();
             const Picked p = pick_digit<THREADS>([&](int i) {
                 uint64_t m = mass[i];
-#pragma unroll
-                for (int c = 1; c < kRowCopies; c++) m += mass[c * kBins + i];
+                for (int c = 1; c < copies; c++) m += mass[c * kBins + i];
                 return m;
-            }, f.above, f.goal, level == 0, set.top_p,
-                                                 waves_u, &pick);
+            }, f.above, f.goal, level == 0, set.top_p, waves_u, &picks[kLevels + level]);
             if (level == 0) f.goal = set.top_p * (double)p.total;
             if (p.digit == kBins) {            // (nothing weighs anything in fixed point but the first)
                 f.done = 1;
@@ -445,14 +459,14 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
             }
             f.found |= p.digit << digit_shift(level);
             f.above = p.above;
-            have = count[p.digit];
-            __syncthreads();
+            if (last) have = count[p.digit];
         }
         if (!f.done) {
             thr = f.found;
             ties = ties_for(f.above, f.goal, weight<DT, OPACITY>(thr, s), a.unit, have);
         }
     }
+    __syncthreads();
     // what is kept: ties by their rank in index order
     uint32_t rank = 0;
     if (thr) {
@@ -496,7 +510,6 @@ constexpr int kSeg = 8;                        // entries between two stored run
 constexpr int kChunkThreads = 256;
 constexpr int kChunk = kChunkThreads * 2 * kSeg;
 constexpr int kChunkSegs = kChunk / kSeg;
-constexpr int kLevels = 3;
 constexpr int kHistThreads = 1024;
 constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
 constexpr int kCopies = 4;
