@@ -507,9 +507,9 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
 
 // ---- longer rows ------------------------------------------------------------------------------------------------------
 constexpr int kSeg = 8;                        // entries between two stored running sums
-constexpr int kChunkThreads = 256;
-constexpr int kChunk = kChunkThreads * 2 * kSeg;
-constexpr int kChunkSegs = kChunk / kSeg;
+constexpr int kChunkThreads = 512;             // (8 entries a thread: a million entries are two waves a SIMD)
+constexpr int kChunk = kChunkThreads * kSeg;
+constexpr int kChunkSegs = kChunkThreads;
 constexpr int kHistThreads = 1024;
 constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
 constexpr int kCopies = 4;
@@ -554,7 +554,7 @@ k_long_max(SampleArgs a, LongArgs g) {
     const char *row = row_base<DT>(a, r);
     uint32_t mx = 0;
 #pragma unroll
-    for (int q = 0; q < 2 * kSeg / kVec<DT>; q++) {
+    for (int q = 0; q < kSeg / kVec<DT>; q++) {
         uint32_t k[kVec<DT>];
         keys_at<DT>(row, (int64_t)c * kChunk + ((int64_t)q * kChunkThreads + tid) * kVec<DT>, a.cols, k);
 #pragma unroll
@@ -563,7 +563,11 @@ k_long_max(SampleArgs a, LongArgs g) {
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
     if ((tid & 63) == 0) waves[tid >> 6] = mx;
     __syncthreads();
-    if (tid == 0) g.chunk_max[(size_t)r * g.chunks + c] = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < kChunkThreads / 64; w++) mx = max(mx, waves[w]);
+        g.chunk_max[(size_t)r * g.chunks + c] = mx;
+    }
 }
 
 // The row's settings and maximum, nothing cut yet.
@@ -824,13 +828,13 @@ __global__ void __launch_bounds__(kChunkThreads)
 k_long_sums(SampleArgs a, LongArgs g) {
     __shared__ uint64_t waves_u[kChunkThreads / 64];
     __shared__ uint32_t waves_i[kChunkThreads / 64];
-    __shared__ uint32_t keys[CUT ? 2 * kSeg : 1][kChunkThreads];
+    __shared__ uint32_t keys[CUT ? kSeg : 1][kChunkThreads];
     const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
     const char *row = row_base<DT>(a, r);
-    const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * 2 * kSeg;
-    uint32_t key[2 * kSeg];
+    const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * kSeg;
+    uint32_t key[kSeg];
 #pragma unroll
-    for (int q = 0; q < 2 * kSeg / kVec<DT>; q++) {
+    for (int q = 0; q < kSeg / kVec<DT>; q++) {
         uint32_t k[kVec<DT>];
         keys_at<DT>(row, i0 + q * kVec<DT>, a.cols, k);
 #pragma unroll
@@ -857,50 +861,48 @@ k_long_sums(SampleArgs a, LongArgs g) {
         ok = st.ok;
         if (c == 0 && tid == 0) g.rows[r] = st;
     }
-    uint64_t sum[2] = {0, 0};
-    uint32_t ties[2] = {0, 0};
+    uint64_t sum = 0;
+    uint32_t ties = 0;
     if (ok) {
         uint32_t above = 0;
 #pragma unroll
-        for (int e = 0; e < 2 * kSeg; e++) {
-            if (CUT && thr) ties[e / kSeg] += key[e] == thr;
+        for (int e = 0; e < kSeg; e++) {
+            if (CUT && thr) ties += key[e] == thr;
             above |= (key[e] > thr && (!greedy || key[e] == s.top)) ? 1u << e : 0u;
         }
         if constexpr (CUT) {
             // A lane goes through its own kept entries: behind a cut a wave takes as many rounds as its fullest lane has,
-            // not sixteen with a few lanes each.
+            // not eight with a few lanes each.
 #pragma unroll
-            for (int e = 0; e < 2 * kSeg; e++) keys[e][tid] = key[e];
+            for (int e = 0; e < kSeg; e++) keys[e][tid] = key[e];
             while (above) {
                 const int e = __builtin_ctz(above);
                 above &= above - 1;
                 const double w = weight<DT, OPACITY>(keys[e][tid], s);
-                if (w >= min_p) sum[e >= kSeg ? 1 : 0] += fixed(w, a.unit);
+                if (w >= min_p) sum += fixed(w, a.unit);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 2 * kSeg; e++) {
+            for (int e = 0; e < kSeg; e++) {
                 const double w = weight<DT, OPACITY>(key[e], s);
-                if (((above >> e) & 1u) && w >= min_p) sum[e / kSeg] += fixed(w, a.unit);
+                if (((above >> e) & 1u) && w >= min_p) sum += fixed(w, a.unit);
             }
         }
     }
     if constexpr (CUT) {                       // (as if all ties were kept: see ChunkView)
-        sum[0] += tie_weight * ties[0];
-        sum[1] += tie_weight * ties[1];
+        sum += tie_weight * ties;
     }
-    const size_t at = (size_t)r * g.chunks + c, seg = at * kChunkSegs + 2 * tid;
+    const size_t at = (size_t)r * g.chunks + c, seg = at * kChunkSegs + tid;
     uint64_t total;
-    const uint64_t before = block_scan<kChunkThreads>(sum[0] + sum[1], waves_u, total);
-    *reinterpret_cast<ulonglong2 *>(g.seg_sum + seg) = make_ulonglong2(before, before + sum[0]);
-    if ((tid & 3) == 0) g.mid_sum[at * (kChunkSegs / 8) + (tid >> 2)] = before;
-    if ((tid & 31) == 0) g.top_sum[at * (kChunkSegs / 64) + (tid >> 5)] = before;
+    const uint64_t before = block_scan<kChunkThreads>(sum, waves_u, total);
+    g.seg_sum[seg] = before;
+    if ((tid & 7) == 0) g.mid_sum[at * (kChunkSegs / 8) + (tid >> 3)] = before;
+    if ((tid & 63) == 0) g.top_sum[at * (kChunkSegs / 64) + (tid >> 6)] = before;
     if (tid == 0) g.chunk_sum[at] = total;
     if constexpr (CUT) {
         if (thr) {
             uint32_t all;
-            const uint32_t ties_before = block_scan<kChunkThreads>(ties[0] + ties[1], waves_i, all);
-            *reinterpret_cast<uint2 *>(g.seg_ties + seg) = make_uint2(ties_before, ties_before + ties[0]);
+            g.seg_ties[seg] = block_scan<kChunkThreads>(ties, waves_i, all);
             if (tid == 0) g.chunk_ties[at] = all;
         }
     }
