@@ -944,19 +944,22 @@ k_long_scan(LongArgs g) {
 }
 
 // A draw is made by LANES neighbouring lanes.  The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not
-// exceed `goal`, LANES values at a time; each of the lanes gets it.
+// exceed `goal`, LANES values at a time; each of the lanes gets it, and its value.
 template <int LANES>
 static __device__ __forceinline__ uint64_t group_ballot(bool b) {
     const uint64_t m = __builtin_amdgcn_ballot_w64(b) >> (threadIdx.x & 63 & ~(LANES - 1));
     return LANES == 64 ? m : m & ((1ull << (LANES & 63)) - 1ull);
 }
 template <int LANES, typename F>
-static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f) {
+static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f, uint64_t &value) {
     const int lane = threadIdx.x & (LANES - 1);
     int lo = 0;
+    value = 0;
     while (n > 1) {                            // (n is the same in every lane of the wave)
         const int step = (n + LANES - 1) / LANES, at = lane * step;
-        const int c = __builtin_popcountll(group_ballot<LANES>(at < n && f(lo + at, step) <= goal)) - 1;   // (f(lo) <= goal)
+        const uint64_t v = at < n ? f(lo + at, step) : ~0ull;
+        const int c = __builtin_popcountll(group_ballot<LANES>(v <= goal)) - 1;   // (f(lo) <= goal)
+        value = __shfl(v, (threadIdx.x & 63 & ~(LANES - 1)) + c, 64);
         lo += c * step;
         n = step;
     }
@@ -1020,11 +1023,12 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     const bool none = total == 0 || isnan(u), greedy = st.greedy;
     const uint64_t goal = (greedy || none) ? 0ull : goal_of(u, total);
     const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-    const int lo = last_not_above<LANES>(g.chunks, goal, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; });
-    const uint64_t rest = goal - chunk_sum[lo];
+    uint64_t before;
+    const int lo = last_not_above<LANES>(g.chunks, goal, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; },
+                                         before);
+    const uint64_t rest = goal - before;
     const ChunkView<CUT> v(g, st, r, lo);
-    const int seg = last_not_above<LANES>(kChunkSegs, rest, [&](int i, int step) { return v.sum_before(i, step); });
-    const uint64_t before = v.sum_before(seg, 1);
+    const int seg = last_not_above<LANES>(kChunkSegs, rest, [&](int i, int step) { return v.sum_before(i, step); }, before);
     const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
     uint32_t key = 0;
     if (lane < kSeg && i0 + lane < a.cols) key = key_at<DT>(row_base<DT>(a, r), i0 + lane);
