@@ -546,6 +546,7 @@ static __device__ __forceinline__ const char *row_base(const SampleArgs &a, int 
     return static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
 }
 
+// A chunk's maximum; the row's histograms are emptied on the way.
 template <int DT>
 __global__ void __launch_bounds__(kChunkThreads)
 k_long_max(SampleArgs a, LongArgs g) {
@@ -559,6 +560,13 @@ k_long_max(SampleArgs a, LongArgs g) {
         keys_at<DT>(row, (int64_t)c * kChunk + ((int64_t)q * kChunkThreads + tid) * kVec<DT>, a.cols, k);
 #pragma unroll
         for (int e = 0; e < kVec<DT>; e++) mx = max(mx, k[e]);
+    }
+    if (g.with_k || g.with_p) {
+        for (int b = c * kChunkThreads + tid; b < kUsedLevels<DT> * kBins; b += g.chunks * kChunkThreads) {
+            if (g.with_k) g.k_count[(size_t)r * kLevels * kBins + b] = 0;
+            if (g.with_p) g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
+            if (g.with_p && b < kBins) g.p_count[(size_t)r * kBins + b] = 0;
+        }
     }
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
     if ((tid & 63) == 0) waves[tid >> 6] = mx;
@@ -602,21 +610,13 @@ static __device__ __forceinline__ uint32_t row_max(const LongArgs &g, int r, uin
     return mx;
 }
 
-// One workgroup per row: its state, empty histograms.
+// One workgroup per row: its state.
 template <int DT, bool OPACITY>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_begin(SampleArgs a, LongArgs g) {
     __shared__ uint32_t waves[kHistThreads / 64];
-    const int r = blockIdx.x, tid = threadIdx.x;
-    constexpr int used = kUsedLevels<DT> * kBins;
-    for (int b = tid; b < used; b += kHistThreads) {
-        if (g.with_k) g.k_count[(size_t)r * kLevels * kBins + b] = 0;
-        if (g.with_p) g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
-    }
-    if (g.with_p)
-        for (int b = tid; b < kBins; b += kHistThreads) g.p_count[(size_t)r * kBins + b] = 0;
-    const uint32_t mx = row_max<kHistThreads>(g, r, waves);
-    if (tid == 0) g.rows[r] = long_row<DT, OPACITY>(a, r, mx);
+    const uint32_t mx = row_max<kHistThreads>(g, blockIdx.x, waves);
+    if (threadIdx.x == 0) g.rows[blockIdx.x] = long_row<DT, OPACITY>(a, blockIdx.x, mx);
 }
 
 // The state behind digit `level`, from its histogram; by every workgroup for itself, so that no launch waits for a last
@@ -674,14 +674,16 @@ static __device__ __forceinline__ void finish_k(const LongArgs &g, int r, const 
 }
 
 // The histogram of a digit of the top-k threshold (MASS false) or of the top-p threshold; `parts` workgroups per row.
+// `first_launch`: none has prepared the rows' state, it is made here.
 // Bound by the loads' latency and by fp64: some 40 instructions a weight, 75 for an opacity's power.
 template <int DT, bool OPACITY, bool MASS>
 __global__ void __launch_bounds__(kHistThreads)
-k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
+k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) {
     // Neighbouring values share a first digit, a wave's atomics then hit few words: four copies of the masses, by lane.
     __shared__ uint64_t mass[MASS ? kBins * kCopies : 1];
     __shared__ uint32_t count[kBins];
     __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ uint32_t waves_i[kHistThreads / 64];
     __shared__ Picked pick;
     const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
     LongRow &st = g.rows[r];
@@ -693,7 +695,13 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
     for (int q = 0; q < kBatch; q++) keys_at<DT>(row, first + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
     uint32_t k_thr = 0, k_ties = 0;
     Search f;
-    if constexpr (MASS) {
+    Scale s;
+    if (first_launch) {
+        const LongRow own = long_row<DT, OPACITY>(a, r, row_max<kHistThreads>(g, r, waves_i));
+        if (part == 0 && tid == 0) st = own;
+        f = MASS ? own.p[0] : own.k[0];
+        s = own.scale;
+    } else if constexpr (MASS) {
         if (level == 0) {
             f = st.p[0];
             if (!f.done) {
@@ -715,7 +723,7 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level) {
     if (level > 0 && part == 0 && tid == 0) (MASS ? st.p : st.k)[level] = f;
     if (f.done) return;
     const bool final_level = level == kUsedLevels<DT> - 1;
-    const Scale s = st.scale;
+    if (!first_launch) s = st.scale;
     // Where few entries agree, a wave would compute a weight for a lane or two of every 64: they are queued (in the space
     // of the copies, which such a histogram does without), and taken 64 at a time.
     const bool queued = MASS && (level > 0 || k_thr != 0);
@@ -975,22 +983,29 @@ struct ChunkView {
     uint64_t tie_weight;
     uint32_t thr, left;
     bool cut;
+    __device__ ChunkView(const LongArgs &g, const LongRow &st, size_t chunk, uint32_t left_, bool cut_) {
+        set(g, st, chunk);
+        left = left_;
+        cut = cut_;
+    }
     __device__ ChunkView(const LongArgs &g, const LongRow &st, int r, int c) {
         const size_t chunk = (size_t)r * g.chunks + c;
-        seg_sum = g.seg_sum + chunk * kChunkSegs;
-        mid_sum = g.mid_sum + chunk * (kChunkSegs / 8);
-        top_sum = g.top_sum + chunk * (kChunkSegs / 64);
-        seg_ties = g.seg_ties + chunk * kChunkSegs;
-        tie_weight = 0;
-        thr = CUT ? st.thr : 0u;
+        set(g, st, chunk);
         left = 0xffffffffu;
         cut = false;
         if (CUT && thr) {
-            tie_weight = st.tie_weight;
             const uint32_t before = g.chunk_ties[chunk];
             left = st.ties > before ? st.ties - before : 0u;
             cut = c + 1 == g.chunks || g.chunk_ties[chunk + 1] - before > left;
         }
+    }
+    __device__ void set(const LongArgs &g, const LongRow &st, size_t chunk) {
+        seg_sum = g.seg_sum + chunk * kChunkSegs;
+        mid_sum = g.mid_sum + chunk * (kChunkSegs / 8);
+        top_sum = g.top_sum + chunk * (kChunkSegs / 64);
+        seg_ties = g.seg_ties + chunk * kChunkSegs;
+        thr = CUT ? st.thr : 0u;
+        tie_weight = (CUT && thr) ? st.tie_weight : 0ull;
     }
     // (i a multiple of `step`: neighbours of a step lie side by side, a draw touches a line per step)
     __device__ uint64_t sum_before(int i, int step) const {
@@ -1010,7 +1025,7 @@ struct ChunkView {
 // A workgroup's draws are of one row, so that what a row has in common stays in scalar registers.
 template <int LANES>
 constexpr int kDrawThreads = LANES == 64 ? 64 : 256;
-template <int DT, bool OPACITY, bool CUT, int LANES>
+template <int DT, bool OPACITY, bool CUT, int LANES, bool SCANNED>
 __global__ void __launch_bounds__(kDrawThreads<LANES>)
 k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
     const int r = blockIdx.x / blocks, lane = threadIdx.x & (LANES - 1);
@@ -1018,16 +1033,42 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     // (lanes without a draw repeat the last: a wave's steps are in common)
     const size_t at = (size_t)r * a.draws + min(mine, a.draws - 1);
     const LongRow &st = g.rows[r];
-    const uint64_t total = st.total;
     const float u = uniforms[at];
-    const bool none = total == 0 || isnan(u), greedy = st.greedy;
-    const uint64_t goal = (greedy || none) ? 0ull : goal_of(u, total);
-    const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-    uint64_t before;
-    const int lo = last_not_above<LANES>(g.chunks, goal, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; },
-                                         before);
-    const uint64_t rest = goal - before;
-    const ChunkView<CUT> v(g, st, r, lo);
+    const bool greedy = st.greedy;
+    uint64_t total, before, rest;
+    int lo;
+    uint32_t left = 0xffffffffu;
+    bool cut = false;
+    if constexpr (SCANNED) {
+        total = st.total;
+        rest = (greedy || total == 0 || isnan(u)) ? 0ull : goal_of(u, total);
+        const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
+        lo = last_not_above<LANES>(g.chunks, rest, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; }, before);
+        rest -= before;
+    } else {
+        // up to 64 chunks, whose sums no launch has scanned: a lane each
+        static_assert(SCANNED || LANES == 64, "a wave");
+        const size_t chunk = (size_t)r * g.chunks + lane;
+        const bool in = lane < g.chunks;
+        uint64_t v = in ? g.chunk_sum[chunk] : 0ull;
+        uint32_t chunk_left = 0xffffffffu, here = 0;
+        if (CUT && st.thr) {
+            here = in ? g.chunk_ties[chunk] : 0u;
+            const uint32_t ties_before = wave_scan(here) - here;
+            chunk_left = st.ties > ties_before ? st.ties - ties_before : 0u;
+            if (chunk_left < here) v -= st.tie_weight * (here - chunk_left);
+        }
+        const uint64_t upto = wave_scan(v);
+        total = st.ok ? __shfl(upto, 63, 64) : 0ull;
+        rest = (greedy || total == 0 || isnan(u)) ? 0ull : goal_of(u, total);
+        lo = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(in && upto - v <= rest)) - 1, 0);
+        rest -= __shfl(upto - v, lo, 64);
+        left = (uint32_t)__shfl((int)chunk_left, lo, 64);
+        cut = __shfl((int)(chunk_left < here), lo, 64) != 0;
+    }
+    const bool none = total == 0 || isnan(u);
+    const ChunkView<CUT> v = SCANNED ? ChunkView<CUT>(g, st, r, lo)
+                                     : ChunkView<CUT>(g, st, (size_t)r * g.chunks + lo, left, cut);
     const int seg = last_not_above<LANES>(kChunkSegs, rest, [&](int i, int step) { return v.sum_before(i, step); }, before);
     const int64_t i0 = (int64_t)lo * kChunk + (int64_t)seg * kSeg;
     uint32_t key = 0;
@@ -1090,8 +1131,8 @@ static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids,
     return GS_OK;
 }
 
-// Up to this many chunks (16 M entries) k_long_sums reads the chunks' maxima itself, a few loads a thread; beyond, that
-// would grow with the square of the row.
+// Up to this many chunks (16 M entries) the launch behind k_long_max reads the chunks' maxima itself, a few loads a thread;
+// beyond, that would grow with the square of the row.
 constexpr int kOwnMaxChunks = 4096;
 
 // Up to this many draws a wave each, in fewer steps: 64 draws of 64 rows 4.0 us, a thread each 10.
@@ -1102,7 +1143,7 @@ static int launch_long(const SampleArgs &a, const LongArgs &g, const float *unif
     const dim3 chunks((unsigned)((int64_t)a.rows * g.chunks)), rows(a.rows);
     GS_LAUNCH((k_long_max<DT>), chunks, dim3(kChunkThreads), 0, s, a, g);
     GS_LAUNCH_CHECK();
-    const bool begun = CUT || g.chunks > kOwnMaxChunks;
+    const bool begun = g.chunks > kOwnMaxChunks;
     if (begun) {
         GS_LAUNCH((k_long_begin<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
         GS_LAUNCH_CHECK();
@@ -1115,32 +1156,41 @@ static int launch_long(const SampleArgs &a, const LongArgs &g, const float *unif
         const dim3 grid((unsigned)(parts * a.rows));
         if (g.with_k)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
-                GS_LAUNCH((k_long_digit<DT, OPACITY, false>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
+                GS_LAUNCH((k_long_digit<DT, OPACITY, false>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level,
+                          !begun && level == 0);
                 GS_LAUNCH_CHECK();
             }
         if (g.with_p)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
-                GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level);
+                GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level,
+                          !begun && !g.with_k && level == 0);
                 GS_LAUNCH_CHECK();
             }
         GS_LAUNCH((k_long_cut<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
         GS_LAUNCH_CHECK();
     }
-    if (begun) {
+    if (CUT || begun) {
         GS_LAUNCH((k_long_sums<DT, OPACITY, CUT, true>), chunks, dim3(kChunkThreads), 0, s, a, g);
     } else {
         GS_LAUNCH((k_long_sums<DT, OPACITY, false, false>), chunks, dim3(kChunkThreads), 0, s, a, g);
     }
     GS_LAUNCH_CHECK();
-    GS_LAUNCH((k_long_scan<CUT>), rows, dim3(kHistThreads), 0, s, g);
-    GS_LAUNCH_CHECK();
-    if ((int64_t)a.rows * a.draws <= kWaveDraws) {
-        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 64>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g, a.draws,
-                  uniforms, ids);
+    const bool few = (int64_t)a.rows * a.draws <= kWaveDraws;
+    const bool scanned = !few || g.chunks > 64;
+    if (scanned) {
+        GS_LAUNCH((k_long_scan<CUT>), rows, dim3(kHistThreads), 0, s, g);
+        GS_LAUNCH_CHECK();
+    }
+    if (!scanned) {
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 64, false>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g,
+                  a.draws, uniforms, ids);
+    } else if (few) {
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 64, true>), dim3((unsigned)(a.rows * a.draws)), dim3(64), 0, s, a, g,
+                  a.draws, uniforms, ids);
     } else {
         const int blocks = (int)(((int64_t)a.draws + 31) / 32);
-        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 8>), dim3((unsigned)((int64_t)blocks * a.rows)), dim3(256), 0, s, a, g, blocks,
-                  uniforms, ids);
+        GS_LAUNCH((k_long_draw<DT, OPACITY, CUT, 8, true>), dim3((unsigned)((int64_t)blocks * a.rows)), dim3(256), 0, s, a, g,
+                  blocks, uniforms, ids);
     }
     GS_LAUNCH_CHECK();
     return GS_OK;
