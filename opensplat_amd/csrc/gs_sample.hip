@@ -281,7 +281,7 @@ static __device__ __forceinline__ T block_scan(T v, T *wave_sums /* LDS [THREADS
 }
 
 // The digit in which the running total, from the largest digit down, reaches the goal (kBins: none does).  `bin(i)`: count
-// or mass of digit i.  Every thread of the workgroup gets the digit and what lies above it; called with the histogram
+// or mass of digit i.  Every thread of the workgroup gets the digit and what lies above it (all, if none does); called with the histogram
 // complete, each time with a place `out` of its own.
 struct Picked {
     uint32_t digit;
@@ -312,6 +312,7 @@ static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goa
         }
     }
     __syncthreads();
+    if (out->digit == kBins) return {kBins, above + total, total};
     return {out->digit, out->above, total};
 }
 
@@ -331,51 +332,37 @@ static __device__ __forceinline__ uint64_t goal_of(float u, uint64_t total) {
 // ---- rows of up to 8192 entries ------------------------------------------------------------------------------------
 constexpr int kEach = 8;                       // entries per thread
 
-// One workgroup per row; thread t holds entries 8 t .. 8 t + 7, so that thread order is index order.  Bound by latency: a
-// dozen barriers, and per digit one LDS atomic an entry; the entries are read once.
-template <int DT, bool OPACITY, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
-    // Histograms.  1024 threads: one for every digit, emptied together, which saves two barriers of sixteen waves a digit;
-    // the first digit's masses in copies by lane (neighbouring values share it, a wave's atomics would hit few words).
-    // Fewer threads: one for all, so that many short rows share a compute unit.  The first words also hold, in turn, the
-    // weights of entry 8 t + e at [e][t], 0 if it is not kept; the counts' the running sums.
-    constexpr int kPitch = THREADS + 1, kRowCopies = THREADS >= 1024 ? 4 : 1;
-    constexpr bool kSplit = THREADS >= 1024;
-    constexpr int kFirst = kEach * kPitch > kBins * kRowCopies ? kEach * kPitch : kBins * kRowCopies;
-    __shared__ uint64_t masses[kFirst + (kSplit ? (kLevels - 1) * kBins : 0)];
-    __shared__ uint64_t counts_or_sums[(kSplit ? kLevels + 1 : 1) * kBins / 2];
-    uint32_t *counts = reinterpret_cast<uint32_t *>(counts_or_sums);
-    uint64_t *kept_w = masses, *run_sum = counts_or_sums;
-    __shared__ uint64_t waves_u[THREADS / 64];
-    __shared__ uint32_t waves_i[THREADS / 64];
-    __shared__ Picked picks[2 * kLevels];
-    const int r = blockIdx.x, tid = threadIdx.x, n = a.cols;
-    const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
-    const RowSettings set = row_settings(a, r);
+// A workgroup's memory for the selection among up to 8 THREADS entries.  Histograms: 1024 threads have one for every
+// digit, emptied together, which saves two barriers of sixteen waves a digit, and the first digit's masses in copies by lane
+// (neighbouring values share it, a wave's atomics would hit few words).  Fewer threads: one for all, so that many short
+// rows share a compute unit.  The first words also hold, in turn, the weights of entry 8 t + e at [e][t], 0 if it is not
+// kept; the counts' the running sums.
+template <int THREADS>
+struct RowShared {
+    static constexpr bool kSplit = THREADS >= 1024;
+    static constexpr int kPitch = THREADS + 1, kCopies = THREADS >= 1024 ? 4 : 1;
+    static constexpr int kFirst = kEach * kPitch > kBins * kCopies ? kEach * kPitch : kBins * kCopies;
+    uint64_t masses[kFirst + (kSplit ? (kLevels - 1) * kBins : 0)];
+    uint64_t counts_or_sums[(kSplit ? kLevels + 1 : 1) * kBins / 2];
+    uint64_t waves_u[THREADS / 64];
+    uint32_t waves_i[THREADS / 64];
+    Picked picks[2 * kLevels];
+};
 
-    uint32_t key[kEach];
-#pragma unroll
-    for (int q = 0; q < kEach / kVec<DT>; q++) {
-        uint32_t k[kVec<DT>];
-        keys_at<DT>(row, (int64_t)tid * kEach + q * kVec<DT>, n, k);
-#pragma unroll
-        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
-    }
-    uint32_t mx = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; e++) mx = max(mx, key[e]);
-    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
-    if constexpr (THREADS > 64) {
-        if ((tid & 63) == 0) waves_i[tid >> 6] = mx;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < THREADS / 64; w++) mx = max(mx, waves_i[w]);
-    }
-    if (!set.ok || mx == 0) {
-        for (int j = tid; j < a.draws; j += THREADS) ids[(size_t)r * a.draws + j] = -1;
-        return;
-    }
+// A row's selection and its draws, by one workgroup; thread t holds the keys of entries 8 t .. 8 t + 7, so that thread order
+// is index order.  `mx`: the largest key, not 0.  `f_k`: the search of top-k as it stands before digit `level_k`.  `index(i)`: the index in the row of entry i.
+template <int DT, bool OPACITY, int THREADS, typename F>
+static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSettings &set, int r, const uint32_t (&key)[kEach],
+                                                uint32_t mx, Search f_k, int level_k, RowShared<THREADS> &sh,
+                                                const float *__restrict__ uniforms,
+                                                int32_t *__restrict__ ids, F index) {
+    constexpr bool kSplit = RowShared<THREADS>::kSplit;
+    constexpr int kPitch = RowShared<THREADS>::kPitch, kRowCopies = RowShared<THREADS>::kCopies;
+    constexpr int kFirst = RowShared<THREADS>::kFirst;
+    uint64_t *masses = sh.masses, *kept_w = sh.masses, *run_sum = sh.counts_or_sums, *waves_u = sh.waves_u;
+    uint32_t *counts = reinterpret_cast<uint32_t *>(sh.counts_or_sums), *waves_i = sh.waves_i;
+    Picked *picks = sh.picks;
+    const int tid = threadIdx.x;
     const Scale s = scale_for<DT, OPACITY>(mx, set.inv_t);
     double w[kEach];
 #pragma unroll
@@ -394,8 +381,8 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         __syncthreads();
     }
     if (with_k) {
-        Search f = {0, (double)set.top_k, 0, 0};
-        for (int level = 0; level < kUsedLevels<DT> && !f.done; level++) {
+        Search f = f_k;
+        for (int level = level_k; level < kUsedLevels<DT> && !f.done; level++) {
             uint32_t *count = counts + (kSplit ? level * kBins : 0);
             if (!kSplit) {
                 __syncthreads();
@@ -501,8 +488,43 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         int e = -1;
         do c += kept_w[++e * kPitch + lo];
         while (c <= goal && e < kEach - 1);
-        ids[(size_t)r * a.draws + j] = isnan(u) ? -1 : lo * kEach + e;
+        ids[(size_t)r * a.draws + j] = isnan(u) ? -1 : index(lo * kEach + e);
     }
+}
+
+// One workgroup per row.  Bound by latency: a dozen barriers, and per digit one LDS atomic an entry; the entries are read
+// once.
+template <int DT, bool OPACITY, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+    __shared__ RowShared<THREADS> sh;
+    const int r = blockIdx.x, tid = threadIdx.x, n = a.cols;
+    const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
+    const RowSettings set = row_settings(a, r);
+    uint32_t key[kEach];
+#pragma unroll
+    for (int q = 0; q < kEach / kVec<DT>; q++) {
+        uint32_t k[kVec<DT>];
+        keys_at<DT>(row, (int64_t)tid * kEach + q * kVec<DT>, n, k);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; e++) key[q * kVec<DT> + e] = k[e];
+    }
+    uint32_t mx = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; e++) mx = max(mx, key[e]);
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+    if constexpr (THREADS > 64) {
+        if ((tid & 63) == 0) sh.waves_i[tid >> 6] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) mx = max(mx, sh.waves_i[w]);
+    }
+    if (!set.ok || mx == 0) {
+        for (int j = tid; j < a.draws; j += THREADS) ids[(size_t)r * a.draws + j] = -1;
+        return;
+    }
+    draw_row<DT, OPACITY, THREADS>(a, set, r, key, mx, {0, (double)set.top_k, 0, 0}, 0, sh, uniforms, ids,
+                                   [](int i) { return i; });
 }
 
 // ---- longer rows ------------------------------------------------------------------------------------------------------
@@ -514,16 +536,24 @@ constexpr int kHistThreads = 1024;
 constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
 constexpr int kCopies = 4;
 constexpr int kQueue = 640;                    // keys a wave can have waiting
+constexpr int kListThreads = 1024;
+constexpr int kListMax = kListThreads * kEach; // entries of a row that one workgroup takes over
+constexpr int kListPitch = 32;
+constexpr int kRun = 256;                      // entries of a row that the shortest run in a list spans
+constexpr int kRunMax = 8192;                  // runs of a row
+template <int DT>
+constexpr int kWaveEntries = 64 * kVec<DT>;    // entries of a wave's load: a run
 
 // A row's state between the launches.  A launch reads what earlier ones wrote and writes other fields.
 struct LongRow {
     double inv_t, top_p, min_p;
     Scale scale;
     uint64_t total, tie_weight;
-    Search k[kLevels], p[kLevels];             // as the launch of that digit found it
+    Search k[kLevels], p[kLevels];             // as the launch of that digit found it (a listed row's k[0]: as it left it)
     uint32_t k_thr, k_ties, thr, ties;
     int32_t top_k;
     uint32_t ok, greedy;
+    uint32_t listed;                           // entries in the row's list; 0: the row has none
 };
 
 struct LongArgs {
@@ -531,14 +561,19 @@ struct LongArgs {
     uint32_t *k_count;                         // [rows][kLevels][kBins]
     uint64_t *p_mass;                          // [rows][kLevels][kBins]
     uint32_t *p_count;                         // [rows][kBins], of the last digit
-    uint32_t *chunk_max;                       // [rows][chunks]
+    uint32_t *chunk_max;                       // [rows][chunks], of which `maxima` are used
     uint64_t *chunk_sum;                       // [rows][chunks]: sums, then running sums
     uint32_t *chunk_ties;                      // [rows][chunks]: ties, then running ties
     uint64_t *seg_sum;                         // [rows][chunks][kChunkSegs] running sums inside the chunk
     uint64_t *mid_sum, *top_sum;               // every 8th and every 64th of them again, for the draws' first steps
     uint32_t *seg_ties;                        // [rows][chunks][kChunkSegs]
-    int chunks;
+    uint2 *list;                               // [rows][kListMax]: key, index
+    int32_t *list_index;                       // [rows][kListMax]: in order
+    uint32_t *list_runs;                       // [rows][run_pitch]: a run's place in the list | its entries << 16
+    uint32_t *list_count;                      // [rows][kListPitch], the first of each: a line of its own
+    int chunks, maxima, run_pitch;
     bool with_k, with_p;                       // launches that look for a threshold
+    bool lists;                                // a row's candidates for top-k may be listed
 };
 
 template <int DT>
@@ -546,7 +581,15 @@ static __device__ __forceinline__ const char *row_base(const SampleArgs &a, int 
     return static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
 }
 
-// A chunk's maximum; the row's histograms are emptied on the way.
+template <int DT>
+static __device__ __forceinline__ void empty_p(const LongArgs &g, int r, int from, int step) {
+    for (int b = from; b < kUsedLevels<DT> * kBins; b += step) {
+        g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
+        if (b < kBins) g.p_count[(size_t)r * kBins + b] = 0;
+    }
+}
+
+// A chunk's maximum; the histograms of top-p are emptied on the way.
 template <int DT>
 __global__ void __launch_bounds__(kChunkThreads)
 k_long_max(SampleArgs a, LongArgs g) {
@@ -561,13 +604,7 @@ k_long_max(SampleArgs a, LongArgs g) {
 #pragma unroll
         for (int e = 0; e < kVec<DT>; e++) mx = max(mx, k[e]);
     }
-    if (g.with_k || g.with_p) {
-        for (int b = c * kChunkThreads + tid; b < kUsedLevels<DT> * kBins; b += g.chunks * kChunkThreads) {
-            if (g.with_k) g.k_count[(size_t)r * kLevels * kBins + b] = 0;
-            if (g.with_p) g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
-            if (g.with_p && b < kBins) g.p_count[(size_t)r * kBins + b] = 0;
-        }
-    }
+    if (g.with_p) empty_p<DT>(g, r, c * kChunkThreads + tid, g.chunks * kChunkThreads);
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
     if ((tid & 63) == 0) waves[tid >> 6] = mx;
     __syncthreads();
@@ -590,17 +627,17 @@ static __device__ __forceinline__ LongRow long_row(const SampleArgs &a, int r, u
     s.ok = set.ok && max_key != 0;
     s.greedy = set.greedy;
     s.scale = scale_for<DT, OPACITY>(max_key, set.inv_t);
-    s.k[0].goal = (double)set.top_k;
-    s.k[0].done = set.greedy || !s.ok || set.top_k == 0;
+    s.k[0].goal = set.greedy ? 1.0 : (double)set.top_k;
+    s.k[0].done = !s.ok || (!set.greedy && set.top_k == 0);
     s.p[0].done = set.greedy || !s.ok || !(set.top_p < 1.0);
     return s;
 }
 
-// Maximum over the row's chunks, by every workgroup for itself.
+// Maximum over the row's parts, by every workgroup for itself.
 template <int THREADS>
 static __device__ __forceinline__ uint32_t row_max(const LongArgs &g, int r, uint32_t *waves /* LDS [THREADS / 64] */) {
     uint32_t mx = 0;
-    for (int c = threadIdx.x; c < g.chunks; c += THREADS) mx = max(mx, g.chunk_max[(size_t)r * g.chunks + c]);
+    for (int c = threadIdx.x; c < g.maxima; c += THREADS) mx = max(mx, g.chunk_max[(size_t)r * g.chunks + c]);
     for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = mx;
     __syncthreads();
@@ -610,7 +647,57 @@ static __device__ __forceinline__ uint32_t row_max(const LongArgs &g, int r, uin
     return mx;
 }
 
-// One workgroup per row: its state.
+// With top-k: empty histograms and lists.
+template <int DT>
+__global__ void __launch_bounds__(kHistThreads)
+k_long_empty(LongArgs g, int parts) {
+    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+    const int from = part * kHistThreads + threadIdx.x, step = parts * kHistThreads;
+    for (int b = from; b < kUsedLevels<DT> * kBins; b += step) g.k_count[(size_t)r * kLevels * kBins + b] = 0;
+    if (g.with_p) empty_p<DT>(g, r, from, step);
+    if (g.lists) {
+        for (int b = from; b < g.run_pitch; b += step) g.list_runs[(size_t)r * g.run_pitch + b] = 0;
+        if (from == 0) g.list_count[(size_t)r * kListPitch] = 0;
+    }
+}
+
+// With top-k: a part's maximum and the histogram of the first digit, which needs nothing else.
+template <int DT>
+__global__ void __launch_bounds__(kHistThreads)
+k_long_first(SampleArgs a, LongArgs g, int parts) {
+    __shared__ uint32_t count[kBins];
+    __shared__ uint32_t waves[kHistThreads / 64];
+    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
+    const char *row = row_base<DT>(a, r);
+    const int64_t n = a.cols, step = (int64_t)kHistThreads * kVec<DT>;
+    for (int b = tid; b < kBins; b += kHistThreads) count[b] = 0;
+    __syncthreads();
+    uint32_t mx = 0;
+    for (int64_t i0 = (int64_t)part * kBatch * step; i0 < n; i0 += (int64_t)parts * kBatch * step) {
+        uint32_t k[kBatch][kVec<DT>];
+#pragma unroll
+        for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
+#pragma unroll
+        for (int q = 0; q < kBatch; q++)
+#pragma unroll
+            for (int e = 0; e < kVec<DT>; e++) {
+                mx = max(mx, k[q][e]);
+                if (k[q][e]) atomicAdd(&count[digit_of(k[q][e], 0)], 1u);
+            }
+    }
+    for (int off = 32; off > 0; off >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, off, 64));
+    if ((tid & 63) == 0) waves[tid >> 6] = mx;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < kHistThreads / 64; w++) mx = max(mx, waves[w]);
+        g.chunk_max[(size_t)r * g.chunks + part] = mx;
+    }
+    for (int b = tid; b < kBins; b += kHistThreads)
+        if (count[b]) atomicAdd(&g.k_count[(size_t)r * kLevels * kBins + b], count[b]);
+}
+
+// Without top-k, one workgroup per row: its state.
 template <int DT, bool OPACITY>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_begin(SampleArgs a, LongArgs g) {
@@ -670,11 +757,13 @@ static __device__ __forceinline__ void finish_k(const LongArgs &g, int r, const 
     const Search f = after_k<DT>(g, r, last, st.k[last], waves_u, pick);
     if (f.done) return;
     thr = f.found;
-    ties = (uint32_t)st.top_k - (uint32_t)f.above;
+    ties = (uint32_t)f.goal - (uint32_t)f.above;
 }
 
 // The histogram of a digit of the top-k threshold (MASS false) or of the top-p threshold; `parts` workgroups per row.
-// `first_launch`: none has prepared the rows' state, it is made here.
+// `first_launch`: none has prepared the rows' state, it is made here.  Where the candidates that the first digit leaves fit
+// one workgroup, its second launch lists them instead, and k_long_list goes on with them: the row is read twice, not six
+// or eight times.
 // Bound by the loads' latency and by fp64: some 40 instructions a weight, 75 for an opacity's power.
 template <int DT, bool OPACITY, bool MASS>
 __global__ void __launch_bounds__(kHistThreads)
@@ -683,10 +772,16 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     __shared__ uint64_t mass[MASS ? kBins * kCopies : 1];
     __shared__ uint32_t count[kBins];
     __shared__ uint64_t waves_u[kHistThreads / 64];
-    __shared__ uint32_t waves_i[kHistThreads / 64];
+    __shared__ uint32_t waves_i[kHistThreads / 64 * kBatch];
+    __shared__ uint32_t list_at;
     __shared__ Picked pick;
     const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
     LongRow &st = g.rows[r];
+    if (!first_launch && (MASS ? st.p : st.k)[MASS ? 0 : 1].done) {
+        if (MASS || level == 1 || part != 0 || tid != 0) return;
+        st.k[level] = st.k[1];
+        return;
+    }
     // the first entries are under way while the digit before this one is picked
     const char *row = row_base<DT>(a, r);
     const int64_t n = a.cols, step = (int64_t)kHistThreads * kVec<DT>, first = (int64_t)part * kBatch * step;
@@ -696,11 +791,22 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     uint32_t k_thr = 0, k_ties = 0;
     Search f;
     Scale s;
+    bool listed = false;
     if (first_launch) {
         const LongRow own = long_row<DT, OPACITY>(a, r, row_max<kHistThreads>(g, r, waves_i));
         if (part == 0 && tid == 0) st = own;
         f = MASS ? own.p[0] : own.k[0];
         s = own.scale;
+        if (!MASS && !f.done) {                // (level 1)
+            f = after_k<DT>(g, r, 0, f, waves_u, &pick);
+            const uint64_t n = f.above + (f.done ? 0 : g.k_count[(size_t)r * kLevels * kBins + digit_of(f.found, 0)]);
+            listed = g.lists && n <= kListMax;
+            if (listed && part == 0 && tid == 0) {
+                st.listed = (uint32_t)n;
+                st.k[0] = f;
+                st.p[0].done = 1;
+            }
+        }
     } else if constexpr (MASS) {
         if (level == 0) {
             f = st.p[0];
@@ -718,9 +824,55 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
             f = after_p<DT, OPACITY>(a, g, r, level - 1, st.p[level - 1], st, k_thr, k_ties, waves_u, &pick, &have);
         }
     } else {
-        f = level == 0 ? st.k[0] : after_k<DT>(g, r, level - 1, st.k[level - 1], waves_u, &pick);
+        f = after_k<DT>(g, r, level - 1, st.k[level - 1], waves_u, &pick);
     }
-    if (level > 0 && part == 0 && tid == 0) (MASS ? st.p : st.k)[level] = f;
+    if (level > 0 && part == 0 && tid == 0) {
+        Search *out = (MASS ? st.p : st.k) + level;
+        *out = f;
+        if (listed) out->done = 1;
+    }
+    if constexpr (!MASS) {
+        if (listed) {
+            // a wave's load is a run of the list, its entries in order; a batch's runs stand together, the batches as they
+            // came (a place asked for by every wave: 16 000 atomics on few lines, 65 us for 64 rows)
+            const int lane = tid & 63, wave = tid >> 6;
+            const uint32_t least = max(f.found, 1u);
+            for (int64_t i0 = first; i0 < n; i0 += (int64_t)parts * kBatch * step) {
+                if (i0 != first) {
+#pragma unroll
+                    for (int q = 0; q < kBatch; q++) keys_at<DT>(row, i0 + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
+                }
+                uint32_t in[kBatch], upto[kBatch], all[kBatch];
+#pragma unroll
+                for (int q = 0; q < kBatch; q++) {
+                    in[q] = 0;
+#pragma unroll
+                    for (int e = 0; e < kVec<DT>; e++) in[q] |= k[q][e] >= least ? 1u << e : 0u;
+                    upto[q] = wave_scan((uint32_t)__builtin_popcount(in[q]));
+                    all[q] = (uint32_t)__builtin_amdgcn_readlane((int)upto[q], 63);
+                    if (lane == 0) waves_i[q * (kHistThreads / 64) + wave] = all[q];
+                }
+                __syncthreads();
+                static_assert(kHistThreads / 64 * kBatch <= 64, "a lane each");
+                const uint32_t one = lane < kHistThreads / 64 * kBatch ? waves_i[lane] : 0u, to_one = wave_scan(one);
+                if (tid == 63 && to_one) list_at = atomicAdd(&g.list_count[(size_t)r * kListPitch], to_one);
+                __syncthreads();
+                const uint32_t place = list_at + to_one - one;
+#pragma unroll
+                for (int q = 0; q < kBatch; q++) {
+                    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)place, q * (kHistThreads / 64) + wave);
+                    if (all[q] == 0) continue;
+                    const int64_t i = i0 + q * step + (int64_t)tid * kVec<DT>;
+                    if (lane == 0) g.list_runs[(size_t)r * g.run_pitch + i / kWaveEntries<DT>] = at | all[q] << 16;
+                    uint32_t to = at + upto[q] - __builtin_popcount(in[q]);
+#pragma unroll
+                    for (int e = 0; e < kVec<DT>; e++)
+                        if ((in[q] >> e) & 1u) g.list[(size_t)r * kListMax + to++] = make_uint2(k[q][e], (uint32_t)(i + e));
+                }
+            }
+            return;
+        }
+    }
     if (f.done) return;
     const bool final_level = level == kUsedLevels<DT> - 1;
     if (!first_launch) s = st.scale;
@@ -796,6 +948,48 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     }
 }
 
+// One workgroup per row that has a list: its runs put in order, then the rest as for a short row.
+template <int DT, bool OPACITY>
+__global__ void __launch_bounds__(kListThreads)
+k_long_list(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+    __shared__ RowShared<kListThreads> sh;
+    static_assert((kRunMax + kListMax) * 4 <= sizeof(sh.masses), "runs and keys in the masses' space");
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const LongRow &st = g.rows[r];
+    const int n = (int)st.listed;
+    if (n == 0) return;
+    int32_t *shift = reinterpret_cast<int32_t *>(sh.masses);   // of a run's entries, from the list to the order
+    uint32_t *keys = reinterpret_cast<uint32_t *>(sh.masses) + kRunMax;
+    const uint2 *list = g.list + (size_t)r * kListMax;
+    int32_t *order = g.list_index + (size_t)r * kListMax;
+    uint32_t before = 0;
+    for (int i = tid; i - tid < g.run_pitch; i += kListThreads) {
+        const uint32_t run = i < g.run_pitch ? g.list_runs[(size_t)r * g.run_pitch + i] : 0u;
+        uint32_t all;
+        const uint32_t start = before + block_scan<kListThreads>(run >> 16, sh.waves_i, all);
+        if (i < g.run_pitch) shift[i] = (int32_t)start - (int32_t)(run & 0xffffu);
+        before += all;
+    }
+    __syncthreads();
+    for (int i = tid; i < kListMax; i += kListThreads) {
+        if (i < n) {
+            const uint2 e = list[i];
+            const int at = i + shift[e.y / kWaveEntries<DT>];
+            keys[at] = e.x;
+            order[at] = (int32_t)e.y;
+        } else {
+            keys[i] = 0;
+        }
+    }
+    __syncthreads();
+    uint32_t key[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) key[e] = keys[tid * kEach + e];
+    __syncthreads();
+    draw_row<DT, OPACITY, kListThreads>(a, row_settings(a, r), r, key, st.scale.top, st.k[0], 1, sh, uniforms, ids,
+                                        [&](int i) { return order[i]; });
+}
+
 // One workgroup per row: threshold and ties, once all digits are counted.
 template <int DT, bool OPACITY>
 __global__ void __launch_bounds__(kHistThreads)
@@ -805,6 +999,7 @@ k_long_cut(SampleArgs a, LongArgs g) {
     const int r = blockIdx.x;
     LongRow &st = g.rows[r];
     constexpr int last = kUsedLevels<DT> - 1;
+    if (st.listed) return;
     uint32_t thr = 0, ties = 0;
     if (g.with_p && !st.p[0].done) {
         thr = st.k_thr;
@@ -838,6 +1033,7 @@ k_long_sums(SampleArgs a, LongArgs g) {
     __shared__ uint32_t waves_i[kChunkThreads / 64];
     __shared__ uint32_t keys[CUT ? kSeg : 1][kChunkThreads];
     const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
+    if (CUT && g.rows[r].listed) return;
     const char *row = row_base<DT>(a, r);
     const int64_t i0 = (int64_t)c * kChunk + (int64_t)tid * kSeg;
     uint32_t key[kSeg];
@@ -924,6 +1120,7 @@ k_long_scan(LongArgs g) {
     __shared__ uint32_t waves_i[kHistThreads / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
     LongRow &st = g.rows[r];
+    if (CUT && st.listed) return;
     const size_t first = (size_t)r * g.chunks;
     const bool ok = st.ok;
     const uint32_t thr = CUT ? st.thr : 0u, ties = CUT ? st.ties : 0u;
@@ -1033,6 +1230,7 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     // (lanes without a draw repeat the last: a wave's steps are in common)
     const size_t at = (size_t)r * a.draws + min(mine, a.draws - 1);
     const LongRow &st = g.rows[r];
+    if (CUT && st.listed) return;
     const float u = uniforms[at];
     const bool greedy = st.greedy;
     uint64_t total, before, rest;
@@ -1095,8 +1293,9 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
 constexpr int kRowLimit = 8192;                // longest row of the one-workgroup form
 
 struct SampleLayout {
-    size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, mid_sum, top_sum, seg_ties, total;
-    int chunks;
+    size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, mid_sum, top_sum, seg_ties, list, list_index,
+        list_runs, list_count, total;
+    int chunks, run_pitch;
     SampleLayout(int n_rows, int cols) {
         size_t o = 0;
         auto take = [&](size_t bytes) { size_t r = o; o += (bytes + 255) & ~(size_t)255; return r; };
@@ -1113,6 +1312,11 @@ struct SampleLayout {
         mid_sum = take(n * kChunkSegs);
         top_sum = take(n * kChunkSegs / 8);
         seg_ties = take(n * kChunkSegs * 4);
+        run_pitch = chunks ? (int)min(((int64_t)cols + kRun - 1) / kRun, (int64_t)kRunMax) : 0;
+        list = take(some * kListMax * 8);
+        list_index = take(some * kListMax * 4);
+        list_runs = take(some * run_pitch * 4);
+        list_count = take(some * kListPitch * 4);
         total = o > 0 ? o : 256;
     }
 };
@@ -1139,31 +1343,44 @@ constexpr int kOwnMaxChunks = 4096;
 constexpr int64_t kWaveDraws = 2048;
 
 template <int DT, bool OPACITY, bool CUT>
-static int launch_long(const SampleArgs &a, const LongArgs &g, const float *uniforms, int32_t *ids, hipStream_t s) {
+static int launch_long(const SampleArgs &a, LongArgs g, const float *uniforms, int32_t *ids, hipStream_t s) {
     const dim3 chunks((unsigned)((int64_t)a.rows * g.chunks)), rows(a.rows);
-    GS_LAUNCH((k_long_max<DT>), chunks, dim3(kChunkThreads), 0, s, a, g);
+    // two workgroups per compute unit over all the rows, none without a batch of loads
+    const int64_t batch = (int64_t)kHistThreads * kVec<DT> * kBatch, most = ((int64_t)a.cols + batch - 1) / batch;
+    int64_t parts = (512 + a.rows - 1) / a.rows;
+    if (parts > most) parts = most;
+    const dim3 grid((unsigned)(parts * a.rows));
+    const bool with_k = CUT && g.with_k, begun = !with_k && g.chunks > kOwnMaxChunks;
+    if (with_k) {
+        g.maxima = (int)parts;                 // (a batch is at least a chunk)
+        const int some = parts < 4 ? (int)parts : 4;
+        GS_LAUNCH((k_long_empty<DT>), dim3((unsigned)(some * a.rows)), dim3(kHistThreads), 0, s, g, some);
+        GS_LAUNCH_CHECK();
+        GS_LAUNCH((k_long_first<DT>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts);
+    } else {
+        GS_LAUNCH((k_long_max<DT>), chunks, dim3(kChunkThreads), 0, s, a, g);
+    }
     GS_LAUNCH_CHECK();
-    const bool begun = g.chunks > kOwnMaxChunks;
     if (begun) {
         GS_LAUNCH((k_long_begin<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
         GS_LAUNCH_CHECK();
     }
     if constexpr (CUT) {
-        // two workgroups per compute unit over all the rows, none without a batch of loads
-        const int64_t batch = (int64_t)kHistThreads * kVec<DT> * kBatch, most = ((int64_t)a.cols + batch - 1) / batch;
-        int64_t parts = (512 + a.rows - 1) / a.rows;
-        if (parts > most) parts = most;
-        const dim3 grid((unsigned)(parts * a.rows));
-        if (g.with_k)
-            for (int level = 0; level < kUsedLevels<DT>; level++) {
+        if (with_k) {
+            for (int level = 1; level < kUsedLevels<DT>; level++) {
                 GS_LAUNCH((k_long_digit<DT, OPACITY, false>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level,
-                          !begun && level == 0);
+                          level == 1);
                 GS_LAUNCH_CHECK();
+                if (level == 1 && g.lists) {
+                    GS_LAUNCH((k_long_list<DT, OPACITY>), rows, dim3(kListThreads), 0, s, a, g, uniforms, ids);
+                    GS_LAUNCH_CHECK();
+                }
             }
+        }
         if (g.with_p)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
                 GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level,
-                          !begun && !g.with_k && level == 0);
+                          !begun && !with_k && level == 0);
                 GS_LAUNCH_CHECK();
             }
         GS_LAUNCH((k_long_cut<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
@@ -1202,11 +1419,14 @@ static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *id
     if (L.chunks == 0) return launch_rows<DT, OPACITY>(a, uniforms, ids, s);
     const GsSampleConfig &c = a.cfg;
     const bool with_k = c.top_k_rows || c.top_k > 0, with_p = c.top_p_rows || c.top_p < 1.0f;
+    // a k that no list can hold, where the host knows it, and rows of more runs than a workgroup's table has go without
+    const bool lists = with_k && (c.top_k_rows || c.top_k <= kListMax) && a.cols <= (int64_t)kRunMax * kWaveEntries<DT>;
     const LongArgs g = {(LongRow *)(ws + L.rows), (uint32_t *)(ws + L.k_count), (uint64_t *)(ws + L.p_mass),
                         (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
                         (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint64_t *)(ws + L.mid_sum),
                         (uint64_t *)(ws + L.top_sum), (uint32_t *)(ws + L.seg_ties),
-                        L.chunks, with_k, with_p};
+                        (uint2 *)(ws + L.list), (int32_t *)(ws + L.list_index), (uint32_t *)(ws + L.list_runs),
+                        (uint32_t *)(ws + L.list_count), L.chunks, L.chunks, L.run_pitch, with_k, with_p, lists};
     return with_k || with_p ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
                             : launch_long<DT, OPACITY, false>(a, g, uniforms, ids, s);
 }

@@ -169,6 +169,36 @@ def test_sample_many_rows(shape):
     check_sample(x, u, top_p=p, top_k=k, temperature=0.9)
 
 
+@pytest.mark.parametrize("dt", sorted(DT))
+@pytest.mark.parametrize("size", [(1, 2_097_152), (1, 2_097_153), (1, 4_194_305), (6, 8193), (6, 100_000)])
+def test_sample_top_k_where_few_or_many_candidates_are_left(size, dt):
+    """Top-k rows whose candidates behind the first digit fit one workgroup (8192 entries), just do not, are fewer than k,
+    stand in one place or all over the row; greedy and unlimited rows beside them."""
+    rows, cols = size
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((rows, cols)).astype(np.float32) * 0.1 - 3.0
+    for r in range(rows):
+        top = (8192, 8193, 100, 5000, 8191, 1)[r] if rows > 1 else 3000
+        top = min(top, cols)
+        at = rng.permutation(cols)[:top] if r % 2 == 0 else np.arange(cols - top, cols)
+        x[r, at] = 1.0 + 0.9 * rng.random(top).astype(np.float32)
+    if rows > 1:
+        x[2, 5000:] = -np.inf
+        x[4, :10] = np.nan
+    u = dev(rng.random((rows, 9), dtype=np.float32))
+    ks = np.array([40, 8000, 7000, 4999, 8191, 3][:rows], np.int32)
+    check_sample(dev(x, DT[dt]), u, top_k=dev(ks))
+    check_sample(dev(x, DT[dt]), u, True, top_k=dev(ks), top_p=0.6, temperature=0.4)
+    check_sample(dev(x, DT[dt]), u, top_k=25, min_p=0.7)
+    check_sample(dev(x, DT[dt]), u, top_k=8192)
+    check_sample(dev(x, DT[dt]), u, top_k=8193, top_p=0.9)
+    if rows > 1:
+        t = dev(np.array([1, 0, 0.5, 0, 2, 1], np.float32))
+        k = dev(np.array([0, 5, 1, 9000, 0, 20], np.int32))
+        p = dev(np.array([0.5, 0.5, 0.5, 1, 1, 0], np.float32))
+        check_sample(dev(x, DT[dt]), u, top_k=k, temperature=t, top_p=p)
+
+
 def test_sample_rows_beyond_32_bit_offsets():
     """The last rows start more than 2^31 elements behind the first."""
     rows, cols, stride = 5, 1000, 600_000_000
