@@ -20,14 +20,16 @@
 //
 // Two forms, by the length of a row:
 //   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row)
-//   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*)
+//   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*).  With top-k, rows
+//   whose candidates behind the first digit number 8192 or fewer are listed and go on as a short row does (k_long_list)
 //
-// Measured (kernels, MI355X): 28 entries 4.6 us; 28 rows of 8160 with top-p 17.3 us; 1 M opacities, 50 000 draws 23 us (max
-// 3.3, sums 9.3, scan 3.9, draws 6.5); 5 M opacities at a temperature with top-p, 250 000 draws 126 us (digits 26 + 19 + 12,
-// sums 22, draws 27, the rest 20); 64 rows of 131072 bfloat16 with top-k and top-p 87 us (digits 10 + 11 + 15 + 16, sums
-// 11).  A pass over 5 M entries at the memory's rate is 5 us: the digits and sums of powers are bound by fp64 issue (75
-// instructions an entry, 9 us a pass at the peak rate) and the fixed 8 to 10 us of a launch that picks a digit, reads a
-// row from the caches and adds up a histogram.
+// Measured (kernels, MI355X): 28 entries 4.6 us; 28 rows of 8160 with top-p 15.4 us; 1 M opacities, 50 000 draws 19 us (max
+// 3.0, sums 7.1, scan 1.7, draws 6.8); 5 M opacities at a temperature with top-p, 250 000 draws 123 us (digits 29 + 19 + 12,
+// sums 21, draws 27, the rest 15); 64 rows of 131072 bfloat16 with top-k and top-p 62 us a call (first digit 9, lists 17,
+// the listed rows 21, the launches for others 3 .. 4 each; with all passes over the rows 78).  A pass over 5 M entries at
+// the memory's rate is 5 us: the digits and sums of powers are bound by fp64 issue (75 instructions an entry, 9 us a pass
+// at the peak rate) and the fixed 8 to 10 us of a launch that picks a digit, reads a row from the caches and adds up a
+// histogram.
 #include <math.h>
 
 #include "gs_device.h"
@@ -1218,7 +1220,7 @@ struct ChunkView {
 // A draw: the last chunk, then the last 8 entries, whose running sum does not exceed the goal, then these side by side.
 // (Integer sums: what is found there holds a weight.)  Bound by the latency of some ten dependent loads, which the other
 // draws' hide: eight lanes a draw make 31 000 waves of 250 000 draws, where a thread a draw left four to a SIMD and
-// fetched fifteen lines (50 000 draws 9.6 -> 6.3 us, 250 000 28.5 -> 26.6).
+// fetched fifteen lines (50 000 draws 9.6 -> 6.7 us, 250 000 28.5 -> 26.0).
 // A workgroup's draws are of one row, so that what a row has in common stays in scalar registers.
 template <int LANES>
 constexpr int kDrawThreads = LANES == 64 ? 64 : 256;
