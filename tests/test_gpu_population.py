@@ -199,6 +199,36 @@ def test_sample_top_k_where_few_or_many_candidates_are_left(size, dt):
         check_sample(dev(x, DT[dt]), u, top_k=k, temperature=t, top_p=p)
 
 
+def test_sample_replays_whose_rows_change_between_lists_and_passes():
+    """One captured call of long rows; between its replays the settings and logits change so that the same row is listed in
+    one and goes through all the passes in the next."""
+    from opensplat_amd import cabi
+
+    rng = np.random.default_rng(4)
+    rows, cols = 4, 50_000
+    x, u = logits_of(rng, rows, cols, "f32"), dev(rng.random((rows, 5), dtype=np.float32))
+    k, t, p = (torch.zeros(rows, device="cuda", dtype=d) for d in (torch.int32, torch.float32, torch.float32))
+    kw = dict(top_k=k, temperature=t, top_p=p)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cabi.sample(x, u, **kw)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            ids = cabi.sample(x, u, **kw)
+    for turn in range(5):
+        x.copy_(torch.from_numpy((rng.standard_normal((rows, cols)) * (0.01, 3.0)[turn % 2]).astype(np.float32)))
+        u.copy_(torch.from_numpy(rng.random((rows, 5), dtype=np.float32)))
+        k.copy_(torch.from_numpy(np.roll(np.array([50, 30_000, 0, 1], np.int32), turn)))
+        t.copy_(torch.from_numpy(np.roll(np.array([1, 0.5, 1, 0], np.float32), 2 * turn)))
+        p.copy_(torch.from_numpy(np.roll(np.array([0.9, 1, 0.3, 0.7], np.float32), -turn)))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = ids.clone()
+        assert torch.equal(torch.from_numpy(check_sample(x, u, **kw)).cuda(), got), turn
+
+
 def test_sample_rows_beyond_32_bit_offsets():
     """The last rows start more than 2^31 elements behind the first."""
     rows, cols, stride = 5, 1000, 600_000_000
