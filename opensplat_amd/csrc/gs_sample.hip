@@ -14,23 +14,29 @@
 // Nothing is sorted.
 //
 // Weights are 64-bit: an index is right or wrong, and with 5 million candidates and 250 000 draws a 24-bit weight would
-// move a border across a draw several times in every call.  Their sums are integers: a weight is rounded once, to a
-// multiple of 2^-50 (rows of up to 4096 entries) to 2^-31 (2^31 entries) of the row's largest, so that sums have no
-// order, running sums never decrease, and a histogram's total, a chunk's and a draw's agree to the last bit.
+// move a border across a draw several times in every call.  Their sums are integers: a weight is rounded once, so that
+// sums have no order, running sums never decrease, and a histogram's total, a chunk's and a draw's agree to the last bit.
+//   up to 8192 entries   one word: multiples of 2^-50 of the row's largest (2^-49 beyond 4096 entries)
+//   longer               two words: multiples of 2^-(124 - 2 c), c = ceil log2 cols: 2^-80 at 4 M entries.  One word's 2^-40
+//                        there is not enough: 4 M entries that weigh e^-15 beside a peak are off by 2^-19 each, all the same
+//                        way, and one draw in eight of the tail's lands on another index
 //
 // Two forms, by the length of a row:
 //   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row)
 //   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*).  With top-k, rows
 //   whose candidates behind the first digit number 8192 or fewer are listed and go on as a short row does (k_long_list)
 //
-// Measured (kernels, MI355X): 28 entries 4.6 us; 28 rows of 8160 with top-p 15.4 us; 1 M opacities, 50 000 draws 19 us (max
-// 3.0, sums 7.1, scan 1.7, draws 6.8); 5 M opacities at a temperature with top-p, 250 000 draws 123 us (digits 29 + 19 + 12,
-// sums 21, draws 27, the rest 15); 64 rows of 131072 bfloat16 with top-k and top-p 62 us a call (first digit 9, lists 17,
-// the listed rows 21, the launches for others 3 .. 4 each; with all passes over the rows 78).  A pass over 5 M entries at
-// the memory's rate is 5 us: the digits and sums of powers are bound by fp64 issue (75 instructions an entry, 9 us a pass
+// Measured (kernels, MI355X): 28 entries 4.8 us; 28 rows of 8160 with top-p 14.4 us; 1 M opacities, 50 000 draws 21 us (max
+// 2.9, sums 8.3, scan 2.0, draws 7.8); 5 M opacities at a temperature with top-p, 250 000 draws 127 us (digits 27 + 20 + 10,
+// sums 23, draws 31, the rest 16); 64 rows of 131072 bfloat16 with top-k and top-p 60 us a call (first digit 10, lists 16,
+// the listed rows 20, the launches for others 3 .. 5 each).  The second word of a weight is some 10 % of a long row's time
+// (1 M 18 -> 20 us a call, 5 M 111 -> 116, 64 x 131072 float32 with top-p 70 -> 81).  A pass over 5 M entries at the memory's
+// rate is 5 us: the digits and sums of powers are bound by fp64 issue (75 instructions an entry, 9 us a pass
 // at the peak rate) and the fixed 8 to 10 us of a launch that picks a digit, reads a row from the caches and adds up a
 // histogram.
 #include <math.h>
+
+#include <type_traits>
 
 #include "gs_device.h"
 #include "../../include/gsplat_densify.h"
@@ -43,7 +49,9 @@ struct SampleArgs {
     const void *logits;
     int64_t stride;
     int rows, cols, draws;
-    double unit;                               // a weight of 1 as an integer: 2^50, or less so that cols * unit <= 2^62
+    double unit;                               // one workgroup: a weight of 1 as an integer, 2^50 or 2^49
+    double high;                               // longer rows: 2^bits, cols * high <= 2^62; a weight of 1 is high * high
+    int bits;
     GsSampleConfig cfg;
 };
 
@@ -227,12 +235,50 @@ static __device__ __forceinline__ bool agrees(uint32_t key, uint32_t found, int 
 }
 
 // A search, for top-k (counts) or top-p (masses), as it stands between two digits.
-struct Search {
-    uint64_t above;                            // count or mass over the digits found
-    double goal;                               // count or mass to reach
+template <typename SUM, typename GOAL>
+struct SearchOf {
+    SUM above;                                 // count or mass over the digits found
+    GOAL goal;                                 // count or mass to reach
     uint32_t found;
     uint32_t done;                             // nothing to cut: every candidate is kept
 };
+using Search = SearchOf<uint64_t, double>;
+
+// Masses of the longer rows, in units of 1 / high^2.
+using Mass = unsigned __int128;
+using MassSearch = SearchOf<Mass, Mass>;
+
+// A weight as high * hi + lo, |lo| <= high / 2: sums of either word over a row stay below 2^63, without carries.
+struct Words {
+    uint64_t hi;
+    int64_t lo;
+};
+static __device__ __forceinline__ Words words_of(double w, double high) {
+    const double h = fma(w, high, 0x1p52), l = fma(fma(w, high, -(h - 0x1p52)), high, 0x1.8p52);
+    return {(uint64_t)__double_as_longlong(h) - 0x4330000000000000ull,
+            (int64_t)((uint64_t)__double_as_longlong(l) - 0x4338000000000000ull)};
+}
+static __device__ __forceinline__ Mass mass_of(const Words &v, int bits) { return ((Mass)v.hi << bits) + (Mass)(__int128)v.lo; }
+static __device__ __forceinline__ double as_double(Mass v) { return (double)(uint64_t)(v >> 64) * 0x1p64 + (double)(uint64_t)v; }
+
+// floor (or ceiling) of f * total without a rounding; 0 <= f < 1, total < 2^112
+static __device__ __forceinline__ Mass share_of(Mass total, float f, bool up) {
+    const uint32_t b = __float_as_uint(f) & 0x7FFFFFFFu, e = b >> 23;   // (-0 is 0)
+    const uint64_t m = e ? (b & 0x7FFFFFu) | 0x800000u : b & 0x7FFFFFu;
+    const int k = e ? 150 - (int)e : 149;      // f = m 2^-k, 24 <= k
+    const Mass low = (Mass)(uint64_t)total * m, x = (Mass)(uint64_t)(total >> 64) * m + (uint64_t)(low >> 64);
+    const uint64_t y = (uint64_t)low;          // f * total = (x 2^64 + y) 2^-k, x < 2^73
+    Mass q;
+    bool rest;
+    if (k < 64) {
+        q = (x << (64 - k)) | (y >> k);
+        rest = (y << (64 - k)) != 0;
+    } else {
+        q = x >> (k - 64);
+        rest = y != 0 || x != (q << (k - 64));
+    }
+    return q + (up && rest ? 1u : 0u);
+}
 
 // w * unit <= 2^50, rounded to the nearest integer: the low bits of that number plus 2^52
 static __device__ __forceinline__ uint64_t fixed(double w, double unit) {
@@ -249,63 +295,88 @@ template <int CTRL, int ROWS>
 static __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
     return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
 }
+template <int CTRL, int ROWS>
+static __device__ __forceinline__ Mass from_lane(Mass v) {
+    return (Mass)from_lane<CTRL, ROWS>((uint64_t)v) | (Mass)from_lane<CTRL, ROWS>((uint64_t)(v >> 64)) << 64;
+}
+// A lane's value as one that the wave has in common, in scalar registers: `lane` is in common too.
+static __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+static __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+    return (uint64_t)lane_value((uint32_t)v, lane) | (uint64_t)lane_value((uint32_t)(v >> 32), lane) << 32;
+}
+static __device__ __forceinline__ Mass lane_value(Mass v, int lane) {
+    return (Mass)lane_value((uint64_t)v, lane) | (Mass)lane_value((uint64_t)(v >> 64), lane) << 64;
+}
+static __device__ __forceinline__ Mass shuffle(Mass v, int lane) {
+    return (Mass)__shfl((uint64_t)v, lane, 64) | (Mass)__shfl((uint64_t)(v >> 64), lane, 64) << 64;
+}
 template <typename T>
-static __device__ __forceinline__ T wave_scan(T v) {
+static __device__ __forceinline__ T row_scan(T v) {   // (the steps inside rows of 16)
     v += from_lane<0x111, 0xF>(v);
     v += from_lane<0x112, 0xF>(v);
     v += from_lane<0x114, 0xF>(v);
     v += from_lane<0x118, 0xF>(v);
+    return v;
+}
+template <typename T>
+static __device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
     v += from_lane<0x142, 0xA>(v);
     v += from_lane<0x143, 0xC>(v);
     return v;
 }
 
-// Exclusive scan over the workgroup in thread order, THREADS a multiple of 64; `total` gets the sum.
+// Exclusive scan over the workgroup in thread order, THREADS a multiple of 64 up to 1024; `total` gets the sum.  Each wave
+// scans the waves' sums in its first lanes: added up one after the other they were 16 times eight instructions of every wave
+// where a sum has four words.
 template <int THREADS, typename T>
 static __device__ __forceinline__ T block_scan(T v, T *wave_sums /* LDS [THREADS / 64] */, T &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const T s = wave_scan(v), before = s - v;
     if constexpr (THREADS == 64) {
-        total = __shfl(s, 63, 64);
+        total = lane_value(s, 63);
         return before;
     }
+    static_assert(THREADS <= 1024, "a row of lanes");
     __syncthreads();
     if (lane == 63) wave_sums[wave] = s;
     __syncthreads();
-    T base = T(0), all = T(0);
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) {
-        if (w == wave) base = all;
-        all += wave_sums[w];
-    }
-    total = all;
-    return base + before;
+    const T one = lane < THREADS / 64 ? wave_sums[lane] : T(0), upto = row_scan(one);
+    total = lane_value(upto, THREADS / 64 - 1);
+    return before + lane_value(upto - one, wave);
 }
 
+static __device__ __forceinline__ bool below(uint64_t sum, double goal) { return (double)sum < goal; }
+static __device__ __forceinline__ bool below(Mass sum, Mass goal) { return sum < goal; }
+
 // The digit in which the running total, from the largest digit down, reaches the goal (kBins: none does).  `bin(i)`: count
-// or mass of digit i.  Every thread of the workgroup gets the digit and what lies above it (all, if none does); called with the histogram
-// complete, each time with a place `out` of its own.
-struct Picked {
+// or mass of digit i; `goal_of_total(t)`: the goal, where all the digits together hold t.  Every thread of the workgroup gets
+// the digit and what lies above it (all, if none does); called with the histogram complete, each time with a place `out` of
+// its own.
+template <typename SUM>
+struct PickedOf {
     uint32_t digit;
-    uint64_t above, total;
+    SUM above, total;
 };
-template <int THREADS, typename F>
-static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goal_is_share, double share,
-                                    uint64_t *wave_sums, Picked *out /* LDS */) {
+using Picked = PickedOf<uint64_t>;
+template <int THREADS, typename SUM, typename F, typename G>
+static __device__ PickedOf<SUM> pick_digit(F bin, SUM above, G goal_of_total, SUM *wave_sums, PickedOf<SUM> *out /* LDS */) {
     constexpr int per = kBins / THREADS < 1 ? 1 : kBins / THREADS;
     const int tid = threadIdx.x, high = kBins - 1 - tid * per;
     if (tid == 0) out->digit = kBins;          // (the scan's barriers stand between this and the writer below)
-    uint64_t mine = 0;
+    SUM mine = 0;
 #pragma unroll 4
     for (int j = 0; j < per; j++) mine += bin(high - j);
-    uint64_t total;
-    uint64_t run = above + block_scan<THREADS>(mine, wave_sums, total);
-    const double need = goal_is_share ? share * (double)total : goal;
+    SUM total;
+    SUM run = above + block_scan<THREADS>(mine, wave_sums, total);
+    const auto need = goal_of_total(total);
     // the one thread whose part crosses: its start is below the goal, its end is not
-    if ((double)run < need && (double)(run + mine) >= need && mine > 0) {
+    if (below(run, need) && !below(run + mine, need) && mine > 0) {
         for (int j = 0; j < per; j++) {
-            const uint64_t b = bin(high - j);
-            if (b > 0 && (double)(run + b) >= need) {
+            const SUM b = bin(high - j);
+            if (b > 0 && !below(run + b, need)) {
                 out->digit = (uint32_t)(high - j);
                 out->above = run;
                 break;
@@ -319,16 +390,29 @@ static __device__ Picked pick_digit(F bin, uint64_t above, double goal, bool goa
 }
 
 static __device__ __forceinline__ uint32_t ties_for(uint64_t above, double goal, double tie_weight, double unit,
-                                                    uint64_t have) {
+                                                    uint64_t have) {  // (one word)
     const double w = (double)fixed(tie_weight, unit);
     const double n = w > 0.0 ? ceil((goal - (double)above) / w) : (double)have;
     return (uint32_t)fmin(fmax(n, 1.0), (double)have);
+}
+
+// The least number of ties that reaches the goal, 1 .. have; `tie`: the mass of one
+static __device__ __forceinline__ uint32_t ties_for(Mass above, Mass goal, Mass tie, uint64_t have) {
+    const Mass lack = goal - above;
+    uint64_t n = (uint64_t)fmin(tie > 0 ? as_double(lack) / as_double(tie) : (double)have, (double)have);
+    if (n < 1) n = 1;
+    while (n < have && tie * n < lack) n++;    // (the quotient is good to a few 2^-52: a step or two)
+    while (n > 1 && tie * (n - 1) >= lack) n--;
+    return (uint32_t)n;
 }
 
 // floor(u * total), below total: the running sums that exceed u * total are those that exceed it
 static __device__ __forceinline__ uint64_t goal_of(float u, uint64_t total) {
     const double g = fmax((double)u, 0.0) * (double)total;
     return g < (double)total ? min((uint64_t)g, total - 1) : total - 1;
+}
+static __device__ __forceinline__ Mass goal_of(float u, Mass total) {
+    return u < 1.0f ? share_of(total, fmaxf(u, 0.0f), false) : total - 1;
 }
 
 // ---- rows of up to 8192 entries ------------------------------------------------------------------------------------
@@ -395,8 +479,8 @@ static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSe
             for (int e = 0; e < kEach; e++)
                 if (key[e] != 0 && agrees(key[e], f.found, level)) atomicAdd(&count[digit_of(key[e], level)], 1u);
             __syncthreads();
-            const Picked p = pick_digit<THREADS>([&](int i) { return (uint64_t)count[i]; }, f.above, f.goal, false, 0.0,
-                                                 waves_u, &picks[level]);
+            const Picked p = pick_digit<THREADS>([&](int i) { return (uint64_t)count[i]; }, f.above,
+                                                 [&](uint64_t) { return f.goal; }, waves_u, &picks[level]);
             if (p.digit == kBins) f.done = 1;  // fewer candidates than k
             else f.found |= p.digit << digit_shift(level);
             f.above = p.above;
@@ -440,7 +524,8 @@ static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSe
                 uint64_t m = mass[i];
                 for (int c = 1; c < copies; c++) m += mass[c * kBins + i];
                 return m;
-            }, f.above, f.goal, level == 0, set.top_p, waves_u, &picks[kLevels + level]);
+            }, f.above, [&](uint64_t t) { return level == 0 ? set.top_p * (double)t : f.goal; }, waves_u,
+                                                 &picks[kLevels + level]);
             if (level == 0) f.goal = set.top_p * (double)p.total;
             if (p.digit == kBins) {            // (nothing weighs anything in fixed point but the first)
                 f.done = 1;
@@ -536,8 +621,8 @@ constexpr int kChunk = kChunkThreads * kSeg;
 constexpr int kChunkSegs = kChunkThreads;
 constexpr int kHistThreads = 1024;
 constexpr int kBatch = 2;                      // loads a thread of a digit's launch has in flight
-constexpr int kCopies = 4;
-constexpr int kQueue = 640;                    // keys a wave can have waiting
+constexpr int kCopies = 2;
+constexpr int kQueue = 576;                    // keys a wave can have waiting
 constexpr int kListThreads = 1024;
 constexpr int kListMax = kListThreads * kEach; // entries of a row that one workgroup takes over
 constexpr int kListPitch = 32;
@@ -550,8 +635,9 @@ constexpr int kWaveEntries = 64 * kVec<DT>;    // entries of a wave's load: a ru
 struct LongRow {
     double inv_t, top_p, min_p;
     Scale scale;
-    uint64_t total, tie_weight;
-    Search k[kLevels], p[kLevels];             // as the launch of that digit found it (a listed row's k[0]: as it left it)
+    Mass total, tie_weight;
+    MassSearch p[kLevels];                     // as the launch of that digit found it (a listed row's k[0]: as it left it)
+    Search k[kLevels];
     uint32_t k_thr, k_ties, thr, ties;
     int32_t top_k;
     uint32_t ok, greedy;
@@ -561,13 +647,13 @@ struct LongRow {
 struct LongArgs {
     LongRow *rows;
     uint32_t *k_count;                         // [rows][kLevels][kBins]
-    uint64_t *p_mass;                          // [rows][kLevels][kBins]
+    uint64_t *p_mass;                          // [rows][kLevels][2][kBins]: the high words' sums, the low words'
     uint32_t *p_count;                         // [rows][kBins], of the last digit
     uint32_t *chunk_max;                       // [rows][chunks], of which `maxima` are used
-    uint64_t *chunk_sum;                       // [rows][chunks]: sums, then running sums
+    Mass *chunk_sum;                           // [rows][chunks]: sums, then running sums
     uint32_t *chunk_ties;                      // [rows][chunks]: ties, then running ties
-    uint64_t *seg_sum;                         // [rows][chunks][kChunkSegs] running sums inside the chunk
-    uint64_t *mid_sum, *top_sum;               // every 8th and every 64th of them again, for the draws' first steps
+    Mass *seg_sum;                             // [rows][chunks][kChunkSegs] running sums inside the chunk
+    Mass *mid_sum, *top_sum;                   // every 8th and every 64th of them again, for the draws' first steps
     uint32_t *seg_ties;                        // [rows][chunks][kChunkSegs]
     uint2 *list;                               // [rows][kListMax]: key, index
     int32_t *list_index;                       // [rows][kListMax]: in order
@@ -585,8 +671,8 @@ static __device__ __forceinline__ const char *row_base(const SampleArgs &a, int 
 
 template <int DT>
 static __device__ __forceinline__ void empty_p(const LongArgs &g, int r, int from, int step) {
-    for (int b = from; b < kUsedLevels<DT> * kBins; b += step) {
-        g.p_mass[(size_t)r * kLevels * kBins + b] = 0;
+    for (int b = from; b < kUsedLevels<DT> * 2 * kBins; b += step) {
+        g.p_mass[(size_t)r * kLevels * 2 * kBins + b] = 0;
         if (b < kBins) g.p_count[(size_t)r * kBins + b] = 0;
     }
 }
@@ -715,8 +801,8 @@ static __device__ __forceinline__ Search after_k(const LongArgs &g, int r, int l
                                                  Picked *pick) {
     if (f.done) return f;
     const uint32_t *bins = g.k_count + ((size_t)r * kLevels + level) * kBins;
-    const Picked p = pick_digit<kHistThreads>([&](int i) { return (uint64_t)bins[i]; }, f.above, f.goal, false, 0.0,
-                                              waves_u, pick);
+    const Picked p = pick_digit<kHistThreads>([&](int i) { return (uint64_t)bins[i]; }, f.above,
+                                              [&](uint64_t) { return f.goal; }, waves_u, pick);
     Search next = f;
     if (p.digit == kBins) next.done = 1;       // fewer candidates than k
     else next.found |= p.digit << digit_shift(level);
@@ -724,22 +810,24 @@ static __device__ __forceinline__ Search after_k(const LongArgs &g, int r, int l
     return next;
 }
 template <int DT, bool OPACITY>
-static __device__ __forceinline__ Search after_p(const SampleArgs &a, const LongArgs &g, int r, int level, const Search &f,
-                                                 const LongRow &st, uint32_t k_thr, uint32_t k_ties, uint64_t *waves_u,
-                                                 Picked *pick, uint64_t *have) {
+static __device__ __forceinline__ MassSearch after_p(const SampleArgs &a, const LongArgs &g, int r, int level,
+                                                     const MassSearch &f, const LongRow &st, uint32_t k_thr, uint32_t k_ties,
+                                                     Mass *waves_m, PickedOf<Mass> *pick, uint64_t *have) {
     if (f.done) return f;
     // the ties that top-k left count as one entry of k_ties times the weight
-    uint64_t tied = 0;
+    Mass tied = 0;
     int tied_digit = -1;
     if (k_thr && agrees(k_thr, f.found, level)) {
-        tied = (uint64_t)k_ties * fixed(weight<DT, OPACITY>(k_thr, st.scale), a.unit);
+        tied = k_ties * mass_of(words_of(weight<DT, OPACITY>(k_thr, st.scale), a.high), a.bits);
         tied_digit = (int)digit_of(k_thr, level);
     }
-    const uint64_t *bins = g.p_mass + ((size_t)r * kLevels + level) * kBins;
-    const Picked p = pick_digit<kHistThreads>([&](int i) { return bins[i] + (i == tied_digit ? tied : 0ull); }, f.above,
-                                              f.goal, level == 0, st.top_p, waves_u, pick);
-    Search next = f;
-    if (level == 0) next.goal = st.top_p * (double)p.total;
+    const uint64_t *bins = g.p_mass + ((size_t)r * kLevels + level) * 2 * kBins;
+    const float share = (float)st.top_p;       // (as it was given)
+    const PickedOf<Mass> p = pick_digit<kHistThreads>([&](int i) {
+        return mass_of({bins[i], (int64_t)bins[kBins + i]}, a.bits) + (i == tied_digit ? tied : (Mass)0);
+    }, f.above, [&](Mass t) { return level == 0 ? share_of(t, share, true) : f.goal; }, waves_m, pick);
+    MassSearch next = f;
+    if (level == 0) next.goal = share_of(p.total, share, true);
     if (p.digit == kBins) {
         next.done = 1;
     } else {
@@ -770,16 +858,19 @@ static __device__ __forceinline__ void finish_k(const LongArgs &g, int r, const 
 template <int DT, bool OPACITY, bool MASS>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) {
-    // Neighbouring values share a first digit, a wave's atomics then hit few words: four copies of the masses, by lane.
-    __shared__ uint64_t mass[MASS ? kBins * kCopies : 1];
+    // Neighbouring values share a first digit, a wave's atomics then hit few words: copies of the masses, by lane.
+    constexpr int kMassWords = 2 * kBins * kCopies, kQueuedWords = 2 * kBins + kQueue * (kHistThreads / 64) / 2;
+    __shared__ uint64_t mass[MASS ? (kMassWords > kQueuedWords ? kMassWords : kQueuedWords) : 1];
     __shared__ uint32_t count[kBins];
     __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ Mass waves_m[MASS ? kHistThreads / 64 : 1];
+    __shared__ PickedOf<Mass> pick_m;
     __shared__ uint32_t waves_i[kHistThreads / 64 * kBatch];
     __shared__ uint32_t list_at;
     __shared__ Picked pick;
     const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x;
     LongRow &st = g.rows[r];
-    if (!first_launch && (MASS ? st.p : st.k)[MASS ? 0 : 1].done) {
+    if (!first_launch && (MASS ? st.p[0].done : st.k[1].done)) {
         if (MASS || level == 1 || part != 0 || tid != 0) return;
         st.k[level] = st.k[1];
         return;
@@ -791,15 +882,16 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
 #pragma unroll
     for (int q = 0; q < kBatch; q++) keys_at<DT>(row, first + (int64_t)tid * kVec<DT> + q * step, n, k[q]);
     uint32_t k_thr = 0, k_ties = 0;
-    Search f;
+    std::conditional_t<MASS, MassSearch, Search> f;
     Scale s;
     bool listed = false;
     if (first_launch) {
         const LongRow own = long_row<DT, OPACITY>(a, r, row_max<kHistThreads>(g, r, waves_i));
         if (part == 0 && tid == 0) st = own;
-        f = MASS ? own.p[0] : own.k[0];
         s = own.scale;
-        if (!MASS && !f.done) {                // (level 1)
+        if constexpr (MASS) f = own.p[0];
+        else f = own.k[0];
+        if constexpr (!MASS) if (!f.done) {    // (level 1)
             f = after_k<DT>(g, r, 0, f, waves_u, &pick);
             const uint64_t n = f.above + (f.done ? 0 : g.k_count[(size_t)r * kLevels * kBins + digit_of(f.found, 0)]);
             listed = g.lists && n <= kListMax;
@@ -823,15 +915,19 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
             k_thr = st.k_thr;
             k_ties = st.k_ties;
             uint64_t have;
-            f = after_p<DT, OPACITY>(a, g, r, level - 1, st.p[level - 1], st, k_thr, k_ties, waves_u, &pick, &have);
+            f = after_p<DT, OPACITY>(a, g, r, level - 1, st.p[level - 1], st, k_thr, k_ties, waves_m, &pick_m,
+                                     &have);
         }
     } else {
         f = after_k<DT>(g, r, level - 1, st.k[level - 1], waves_u, &pick);
     }
     if (level > 0 && part == 0 && tid == 0) {
-        Search *out = (MASS ? st.p : st.k) + level;
-        *out = f;
-        if (listed) out->done = 1;
+        if constexpr (MASS) {
+            st.p[level] = f;
+        } else {
+            st.k[level] = f;
+            if (listed) st.k[level].done = 1;
+        }
     }
     if constexpr (!MASS) {
         if (listed) {
@@ -884,7 +980,7 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     const int copies = (MASS && !queued) ? kCopies : 1;
     for (int b = tid; b < kBins; b += kHistThreads) {
         if constexpr (MASS)
-            for (int c = 0; c < copies; c++) mass[b * copies + c] = 0;
+            for (int c = 0; c < 2 * copies; c++) mass[c * kBins + b] = 0;
         count[b] = 0;
     }
     __syncthreads();
@@ -892,15 +988,16 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     auto add = [&](uint32_t key) {
         const uint32_t d = digit_of(key, level);
         if constexpr (MASS) {
-            atomicAdd((unsigned long long *)&mass[d * copies + copy],
-                      (unsigned long long)fixed(weight<DT, OPACITY>(key, s), a.unit));
+            const Words v = words_of(weight<DT, OPACITY>(key, s), a.high);
+            atomicAdd((unsigned long long *)&mass[d * copies + copy], (unsigned long long)v.hi);
+            atomicAdd((unsigned long long *)&mass[(d + kBins) * copies + copy], (unsigned long long)v.lo);
             if (final_level) atomicAdd(&count[d], 1u);
         } else {
             atomicAdd(&count[d], 1u);
         }
     };
-    static_assert(63 + 64 * 8 <= kQueue && kQueue * (kHistThreads / 64) * 4 <= kBins * (kCopies - 1) * 8, "a load's keys and a rest");
-    uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? kBins : 0)) + (tid >> 6) * kQueue;
+    static_assert(63 + 64 * 8 <= kQueue, "a load's keys and a rest");
+    uint32_t *wave_queue = reinterpret_cast<uint32_t *>(mass + (MASS ? 2 * kBins : 0)) + (tid >> 6) * kQueue;
     int waiting = 0;
     for (int64_t i0 = first; i0 < n; i0 += (int64_t)parts * kBatch * step) {
         if (i0 != first) {
@@ -940,9 +1037,14 @@ k_long_digit(SampleArgs a, LongArgs g, int parts, int level, bool first_launch) 
     __syncthreads();
     for (int b = tid; b < kBins; b += kHistThreads) {
         if constexpr (MASS) {
-            uint64_t m = 0;
-            for (int c = 0; c < copies; c++) m += mass[b * copies + c];
-            if (m) atomicAdd((unsigned long long *)&g.p_mass[((size_t)r * kLevels + level) * kBins + b], (unsigned long long)m);
+            uint64_t hi = 0, lo = 0;
+            for (int c = 0; c < copies; c++) {
+                hi += mass[b * copies + c];
+                lo += mass[(b + kBins) * copies + c];
+            }
+            unsigned long long *out = (unsigned long long *)g.p_mass + ((size_t)r * kLevels + level) * 2 * kBins + b;
+            if (hi) atomicAdd(out, (unsigned long long)hi);
+            if (lo) atomicAdd(out + kBins, (unsigned long long)lo);
             if (final_level && count[b]) atomicAdd(&g.p_count[(size_t)r * kBins + b], count[b]);
         } else {
             if (count[b]) atomicAdd(&g.k_count[((size_t)r * kLevels + level) * kBins + b], count[b]);
@@ -997,7 +1099,9 @@ template <int DT, bool OPACITY>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_cut(SampleArgs a, LongArgs g) {
     __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ Mass waves_m[kHistThreads / 64];
     __shared__ Picked pick;
+    __shared__ PickedOf<Mass> pick_m;
     const int r = blockIdx.x;
     LongRow &st = g.rows[r];
     constexpr int last = kUsedLevels<DT> - 1;
@@ -1007,10 +1111,10 @@ k_long_cut(SampleArgs a, LongArgs g) {
         thr = st.k_thr;
         ties = st.k_ties;
         uint64_t have = 0;
-        const Search f = after_p<DT, OPACITY>(a, g, r, last, st.p[last], st, thr, ties, waves_u, &pick, &have);
+        const MassSearch f = after_p<DT, OPACITY>(a, g, r, last, st.p[last], st, thr, ties, waves_m, &pick_m, &have);
         if (!f.done) {
             thr = f.found;
-            ties = ties_for(f.above, f.goal, weight<DT, OPACITY>(thr, st.scale), a.unit, have);
+            ties = ties_for(f.above, f.goal, mass_of(words_of(weight<DT, OPACITY>(thr, st.scale), a.high), a.bits), have);
         }
     } else {
         finish_k<DT>(g, r, st, waves_u, &pick, thr, ties);
@@ -1021,7 +1125,7 @@ k_long_cut(SampleArgs a, LongArgs g) {
         st.tie_weight = 0;
         if (thr) {
             const double w = weight<DT, OPACITY>(thr, st.scale);
-            st.tie_weight = w >= st.min_p ? fixed(w, a.unit) : 0ull;
+            st.tie_weight = w >= st.min_p ? mass_of(words_of(w, a.high), a.bits) : (Mass)0;
         }
     }
 }
@@ -1031,7 +1135,7 @@ k_long_cut(SampleArgs a, LongArgs g) {
 template <int DT, bool OPACITY, bool CUT, bool BEGUN>
 __global__ void __launch_bounds__(kChunkThreads)
 k_long_sums(SampleArgs a, LongArgs g) {
-    __shared__ uint64_t waves_u[kChunkThreads / 64];
+    __shared__ Mass waves_m[kChunkThreads / 64];
     __shared__ uint32_t waves_i[kChunkThreads / 64];
     __shared__ uint32_t keys[CUT ? kSeg : 1][kChunkThreads];
     const int r = blockIdx.x / g.chunks, c = blockIdx.x - r * g.chunks, tid = threadIdx.x;
@@ -1050,11 +1154,11 @@ k_long_sums(SampleArgs a, LongArgs g) {
     double min_p;
     Scale s;
     bool greedy, ok;
-    uint64_t tie_weight = 0;
+    Mass tie_weight = 0;
     if constexpr (BEGUN) {
         const LongRow &st = g.rows[r];
         thr = CUT ? st.thr : 0u;
-        tie_weight = CUT ? st.tie_weight : 0ull;
+        tie_weight = CUT ? st.tie_weight : (Mass)0;
         s = st.scale;
         min_p = st.min_p;
         greedy = st.greedy;
@@ -1067,7 +1171,12 @@ k_long_sums(SampleArgs a, LongArgs g) {
         ok = st.ok;
         if (c == 0 && tid == 0) g.rows[r] = st;
     }
-    uint64_t sum = 0;
+    Words some = {0, 0};
+    auto add = [&](double w) {
+        const Words v = words_of(w, a.high);
+        some.hi += v.hi;
+        some.lo += v.lo;
+    };
     uint32_t ties = 0;
     if (ok) {
         uint32_t above = 0;
@@ -1085,22 +1194,23 @@ k_long_sums(SampleArgs a, LongArgs g) {
                 const int e = __builtin_ctz(above);
                 above &= above - 1;
                 const double w = weight<DT, OPACITY>(keys[e][tid], s);
-                if (w >= min_p) sum += fixed(w, a.unit);
+                if (w >= min_p) add(w);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < kSeg; e++) {
                 const double w = weight<DT, OPACITY>(key[e], s);
-                if (((above >> e) & 1u) && w >= min_p) sum += fixed(w, a.unit);
+                if (((above >> e) & 1u) && w >= min_p) add(w);
             }
         }
     }
+    Mass sum = mass_of(some, a.bits);
     if constexpr (CUT) {                       // (as if all ties were kept: see ChunkView)
         sum += tie_weight * ties;
     }
     const size_t at = (size_t)r * g.chunks + c, seg = at * kChunkSegs + tid;
-    uint64_t total;
-    const uint64_t before = block_scan<kChunkThreads>(sum, waves_u, total);
+    Mass total;
+    const Mass before = block_scan<kChunkThreads>(sum, waves_m, total);
     g.seg_sum[seg] = before;
     if ((tid & 7) == 0) g.mid_sum[at * (kChunkSegs / 8) + (tid >> 3)] = before;
     if ((tid & 63) == 0) g.top_sum[at * (kChunkSegs / 64) + (tid >> 6)] = before;
@@ -1118,7 +1228,7 @@ k_long_sums(SampleArgs a, LongArgs g) {
 template <bool CUT>
 __global__ void __launch_bounds__(kHistThreads)
 k_long_scan(LongArgs g) {
-    __shared__ uint64_t waves_u[kHistThreads / 64];
+    __shared__ Mass waves_m[kHistThreads / 64];
     __shared__ uint32_t waves_i[kHistThreads / 64];
     const int r = blockIdx.x, tid = threadIdx.x;
     LongRow &st = g.rows[r];
@@ -1126,13 +1236,13 @@ k_long_scan(LongArgs g) {
     const size_t first = (size_t)r * g.chunks;
     const bool ok = st.ok;
     const uint32_t thr = CUT ? st.thr : 0u, ties = CUT ? st.ties : 0u;
-    const uint64_t tie_weight = CUT ? st.tie_weight : 0ull;
-    uint64_t base = 0;
+    const Mass tie_weight = CUT ? st.tie_weight : (Mass)0;
+    Mass base = 0;
     uint32_t tie_base = 0;
     for (int c0 = 0; c0 < g.chunks; c0 += kHistThreads) {
         const int c = c0 + tid;
         const bool in = c < g.chunks;
-        uint64_t v = in ? g.chunk_sum[first + c] : 0ull;
+        Mass v = in ? g.chunk_sum[first + c] : (Mass)0;
         if (CUT && thr) {
             const uint32_t here = in ? g.chunk_ties[first + c] : 0u;
             uint32_t all;
@@ -1142,12 +1252,12 @@ k_long_scan(LongArgs g) {
             const uint32_t left = ties > before ? ties - before : 0u;
             if (left < here) v -= tie_weight * (here - left);
         }
-        uint64_t all;
-        const uint64_t before = base + block_scan<kHistThreads>(v, waves_u, all);
+        Mass all;
+        const Mass before = base + block_scan<kHistThreads>(v, waves_m, all);
         base += all;
         if (in) g.chunk_sum[first + c] = before;
     }
-    if (tid == 0) st.total = ok ? base : 0ull;
+    if (tid == 0) st.total = ok ? base : (Mass)0;
 }
 
 // A draw is made by LANES neighbouring lanes.  The last of `n` non-decreasing values f(0) = 0, f(1), ... that does not
@@ -1158,15 +1268,15 @@ static __device__ __forceinline__ uint64_t group_ballot(bool b) {
     return LANES == 64 ? m : m & ((1ull << (LANES & 63)) - 1ull);
 }
 template <int LANES, typename F>
-static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f, uint64_t &value) {
+static __device__ __forceinline__ int last_not_above(int n, Mass goal, F f, Mass &value) {
     const int lane = threadIdx.x & (LANES - 1);
     int lo = 0;
     value = 0;
     while (n > 1) {                            // (n is the same in every lane of the wave)
         const int step = (n + LANES - 1) / LANES, at = lane * step;
-        const uint64_t v = at < n ? f(lo + at, step) : ~0ull;
+        const Mass v = at < n ? f(lo + at, step) : ~(Mass)0;
         const int c = __builtin_popcountll(group_ballot<LANES>(v <= goal)) - 1;   // (f(lo) <= goal)
-        value = __shfl(v, (threadIdx.x & 63 & ~(LANES - 1)) + c, 64);
+        value = shuffle(v, (threadIdx.x & 63 & ~(LANES - 1)) + c);
         lo += c * step;
         n = step;
     }
@@ -1177,9 +1287,9 @@ static __device__ __forceinline__ int last_not_above(int n, uint64_t goal, F f, 
 // ones behind the `left` first are taken off.
 template <bool CUT>
 struct ChunkView {
-    const uint64_t *seg_sum, *mid_sum, *top_sum;
+    const Mass *seg_sum, *mid_sum, *top_sum;
     const uint32_t *seg_ties;
-    uint64_t tie_weight;
+    Mass tie_weight;
     uint32_t thr, left;
     bool cut;
     __device__ ChunkView(const LongArgs &g, const LongRow &st, size_t chunk, uint32_t left_, bool cut_) {
@@ -1204,11 +1314,11 @@ struct ChunkView {
         top_sum = g.top_sum + chunk * (kChunkSegs / 64);
         seg_ties = g.seg_ties + chunk * kChunkSegs;
         thr = CUT ? st.thr : 0u;
-        tie_weight = (CUT && thr) ? st.tie_weight : 0ull;
+        tie_weight = (CUT && thr) ? st.tie_weight : (Mass)0;
     }
     // (i a multiple of `step`: neighbours of a step lie side by side, a draw touches a line per step)
-    __device__ uint64_t sum_before(int i, int step) const {
-        uint64_t v = step == 64 ? top_sum[i >> 6] : (step == 8 ? mid_sum[i >> 3] : seg_sum[i]);
+    __device__ Mass sum_before(int i, int step) const {
+        Mass v = step == 64 ? top_sum[i >> 6] : (step == 8 ? mid_sum[i >> 3] : seg_sum[i]);
         if (CUT && cut) {
             const uint32_t t = seg_ties[i];
             if (t > left) v -= tie_weight * (t - left);
@@ -1220,7 +1330,7 @@ struct ChunkView {
 // A draw: the last chunk, then the last 8 entries, whose running sum does not exceed the goal, then these side by side.
 // (Integer sums: what is found there holds a weight.)  Bound by the latency of some ten dependent loads, which the other
 // draws' hide: eight lanes a draw make 31 000 waves of 250 000 draws, where a thread a draw left four to a SIMD and
-// fetched fifteen lines (50 000 draws 9.6 -> 6.7 us, 250 000 28.5 -> 26.0).
+// fetched fifteen lines (with sums of one word 50 000 draws 9.6 -> 6.7 us, 250 000 28.5 -> 26.0; of two 7.8 and 31).
 // A workgroup's draws are of one row, so that what a row has in common stays in scalar registers.
 template <int LANES>
 constexpr int kDrawThreads = LANES == 64 ? 64 : 256;
@@ -1235,22 +1345,22 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     if (CUT && st.listed) return;
     const float u = uniforms[at];
     const bool greedy = st.greedy;
-    uint64_t total, before, rest;
+    Mass total, before, rest;
     int lo;
     uint32_t left = 0xffffffffu;
     bool cut = false;
     if constexpr (SCANNED) {
         total = st.total;
-        rest = (greedy || total == 0 || isnan(u)) ? 0ull : goal_of(u, total);
-        const uint64_t *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
-        lo = last_not_above<LANES>(g.chunks, rest, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~0ull; }, before);
+        rest = (greedy || total == 0 || isnan(u)) ? (Mass)0 : goal_of(u, total);
+        const Mass *chunk_sum = g.chunk_sum + (size_t)r * g.chunks;
+        lo = last_not_above<LANES>(g.chunks, rest, [&](int i, int) { return i < g.chunks ? chunk_sum[i] : ~(Mass)0; }, before);
         rest -= before;
     } else {
         // up to 64 chunks, whose sums no launch has scanned: a lane each
         static_assert(SCANNED || LANES == 64, "a wave");
         const size_t chunk = (size_t)r * g.chunks + lane;
         const bool in = lane < g.chunks;
-        uint64_t v = in ? g.chunk_sum[chunk] : 0ull;
+        Mass v = in ? g.chunk_sum[chunk] : (Mass)0;
         uint32_t chunk_left = 0xffffffffu, here = 0;
         if (CUT && st.thr) {
             here = in ? g.chunk_ties[chunk] : 0u;
@@ -1258,11 +1368,11 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
             chunk_left = st.ties > ties_before ? st.ties - ties_before : 0u;
             if (chunk_left < here) v -= st.tie_weight * (here - chunk_left);
         }
-        const uint64_t upto = wave_scan(v);
-        total = st.ok ? __shfl(upto, 63, 64) : 0ull;
-        rest = (greedy || total == 0 || isnan(u)) ? 0ull : goal_of(u, total);
+        const Mass upto = wave_scan(v);
+        total = st.ok ? shuffle(upto, 63) : (Mass)0;
+        rest = (greedy || total == 0 || isnan(u)) ? (Mass)0 : goal_of(u, total);
         lo = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(in && upto - v <= rest)) - 1, 0);
-        rest -= __shfl(upto - v, lo, 64);
+        rest -= shuffle(upto - v, lo);
         left = (uint32_t)__shfl((int)chunk_left, lo, 64);
         cut = __shfl((int)(chunk_left < here), lo, 64) != 0;
     }
@@ -1277,14 +1387,14 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
     uint32_t rank = 0;                         // (where nothing is cut, every rank is below `left`)
     if (CUT && v.cut) rank = v.seg_ties[seg];
     rank += __builtin_popcountll(group_ballot<LANES>(tied) & ((1ull << lane) - 1ull));
-    uint64_t run = 0;
+    Mass run = 0;
     if ((key > v.thr || (tied && rank < v.left)) && (!greedy || key == st.scale.top)) {
         const double w = weight<DT, OPACITY>(key, st.scale);
-        if (w >= st.min_p) run = fixed(w, a.unit);
+        if (w >= st.min_p) run = mass_of(words_of(w, a.high), a.bits);
     }
 #pragma unroll
     for (int off = 1; off < kSeg; off <<= 1) {
-        const uint64_t o = __shfl_up(run, off, 64);
+        const Mass o = shuffle(run, (threadIdx.x - off) & 63);
         if (lane >= off) run += o;
     }
     const uint64_t over = group_ballot<LANES>(lane < kSeg && before + run > rest);
@@ -1305,14 +1415,14 @@ struct SampleLayout {
         const size_t n = (size_t)n_rows * chunks, some = chunks ? (size_t)n_rows : 0;
         rows = take(some * sizeof(LongRow));
         k_count = take(some * kLevels * kBins * 4);
-        p_mass = take(some * kLevels * kBins * 8);
+        p_mass = take(some * kLevels * 2 * kBins * 8);
         p_count = take(some * kBins * 4);
         chunk_max = take(n * 4);
-        chunk_sum = take(n * 8);
+        chunk_sum = take(n * sizeof(Mass));
         chunk_ties = take(n * 4);
-        seg_sum = take(n * kChunkSegs * 8);
-        mid_sum = take(n * kChunkSegs);
-        top_sum = take(n * kChunkSegs / 8);
+        seg_sum = take(n * kChunkSegs * sizeof(Mass));
+        mid_sum = take(n * kChunkSegs / 8 * sizeof(Mass));
+        top_sum = take(n * kChunkSegs / 64 * sizeof(Mass));
         seg_ties = take(n * kChunkSegs * 4);
         run_pitch = chunks ? (int)min(((int64_t)cols + kRun - 1) / kRun, (int64_t)kRunMax) : 0;
         list = take(some * kListMax * 8);
@@ -1352,6 +1462,10 @@ static int launch_long(const SampleArgs &a, LongArgs g, const float *uniforms, i
     int64_t parts = (512 + a.rows - 1) / a.rows;
     if (parts > most) parts = most;
     const dim3 grid((unsigned)(parts * a.rows));
+    // One for the masses: every workgroup adds its two words of up to 2048 bins to the row's (calls of 5 M opacities and of
+    // 64 x 131072 with top-p: 256 workgroups 116 and 81 us, 512 for the first digit 119 and 83, for all of them 135 and 102,
+    // 128 behind the first 129 and 98)
+    const int64_t fewer = (256 + a.rows - 1) / a.rows, mass_parts = fewer < parts ? fewer : parts;
     const bool with_k = CUT && g.with_k, begun = !with_k && g.chunks > kOwnMaxChunks;
     if (with_k) {
         g.maxima = (int)parts;                 // (a batch is at least a chunk)
@@ -1381,8 +1495,8 @@ static int launch_long(const SampleArgs &a, LongArgs g, const float *uniforms, i
         }
         if (g.with_p)
             for (int level = 0; level < kUsedLevels<DT>; level++) {
-                GS_LAUNCH((k_long_digit<DT, OPACITY, true>), grid, dim3(kHistThreads), 0, s, a, g, (int)parts, level,
-                          !begun && !with_k && level == 0);
+                GS_LAUNCH((k_long_digit<DT, OPACITY, true>), dim3((unsigned)(mass_parts * a.rows)), dim3(kHistThreads), 0, s, a, g,
+                          (int)mass_parts, level, !begun && !with_k && level == 0);
                 GS_LAUNCH_CHECK();
             }
         GS_LAUNCH((k_long_cut<DT, OPACITY>), rows, dim3(kHistThreads), 0, s, a, g);
@@ -1424,9 +1538,9 @@ static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *id
     // a k that no list can hold, where the host knows it, and rows of more runs than a workgroup's table has go without
     const bool lists = with_k && (c.top_k_rows || c.top_k <= kListMax) && a.cols <= (int64_t)kRunMax * kWaveEntries<DT>;
     const LongArgs g = {(LongRow *)(ws + L.rows), (uint32_t *)(ws + L.k_count), (uint64_t *)(ws + L.p_mass),
-                        (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (uint64_t *)(ws + L.chunk_sum),
-                        (uint32_t *)(ws + L.chunk_ties), (uint64_t *)(ws + L.seg_sum), (uint64_t *)(ws + L.mid_sum),
-                        (uint64_t *)(ws + L.top_sum), (uint32_t *)(ws + L.seg_ties),
+                        (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (Mass *)(ws + L.chunk_sum),
+                        (uint32_t *)(ws + L.chunk_ties), (Mass *)(ws + L.seg_sum), (Mass *)(ws + L.mid_sum),
+                        (Mass *)(ws + L.top_sum), (uint32_t *)(ws + L.seg_ties),
                         (uint2 *)(ws + L.list), (int32_t *)(ws + L.list_index), (uint32_t *)(ws + L.list_runs),
                         (uint32_t *)(ws + L.list_count), L.chunks, L.chunks, L.run_pitch, with_k, with_p, lists};
     return with_k || with_p ? launch_long<DT, OPACITY, true>(a, g, uniforms, ids, s)
@@ -1464,10 +1578,12 @@ extern "C" int gs_sample(int rows, int cols, const void *logits, int64_t row_str
         (L.chunks && (int64_t)rows * (((int64_t)draws + 31) / 32) > 0xffffffffLL / 256))
         return GS_ERR_UNSUPPORTED;
     if (workspace_bytes < L.total) return GS_ERR_WORKSPACE;
-    SampleArgs a = {logits, row_stride, rows, cols, draws, 0.0, *cfg};
-    int log_cols = 0;
+    int log_cols = 12;
     while (((int64_t)1 << log_cols) < cols) log_cols++;
-    a.unit = ldexp(1.0, log_cols < 12 ? 50 : 62 - log_cols);
+    const int bits = 62 - log_cols;
+    // (a list holds kListMax entries at most, whatever the row's length)
+    static_assert(kListMax == 8192 && kRowLimit == 8192, "sums of 2^13 weights of 2^49");
+    const SampleArgs a = {logits, row_stride, rows, cols, draws, ldexp(1.0, log_cols == 12 ? 50 : 49), ldexp(1.0, bits), bits, *cfg};
     const bool op = cfg->flags & GS_FLAG_LOGIT_OPACITY;
     hipStream_t s = (hipStream_t)stream;
     char *ws = (char *)workspace;

@@ -102,3 +102,34 @@ def relocate(params, exp_avg, exp_avg_sq, targets, sources, min_opacity):
             a[t] = 0
             a[drawn] = 0
     return p, moments[0], moments[1]
+
+
+def running(w):
+    """Running sums in longdouble, a block's inside it and the blocks' before it: each has seen some 2 sqrt(n) roundings of
+    2^-64, not n of them all the same way."""
+    side = int(np.ceil(np.sqrt(max(len(w), 1))))
+    a = np.zeros(side * side, np.longdouble)
+    a[:len(w)] = w
+    a = np.cumsum(a.reshape(side, side), 1)
+    a[1:] += np.cumsum(a[:-1, -1])[:, None]
+    return a.reshape(-1)[:len(w)]
+
+
+def kept_weights(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, opacity=False):
+    """What sample_row draws from, no weight rounded: the kept indices of a row x [V] in ascending order and their weights
+    (the largest is 1)."""
+    x = np.asarray(x, np.float64)
+    at = np.flatnonzero(x > -np.inf)
+    v = x[at].astype(np.longdouble)
+    if opacity:
+        v = -np.logaddexp(np.longdouble(0), -v)
+    w = np.exp((v - v.max()) / np.longdouble(np.float32(temperature)))   # (as the C ABI takes it)
+    order = np.argsort(-x[at], kind="stable")
+    if top_k > 0:
+        order = order[:top_k]
+    if top_p < 1.0:
+        mass = running(w[order])
+        order = order[:1 + int(np.searchsorted(mass, np.longdouble(np.float32(top_p)) * mass[-1]))]
+    kept = np.sort(order)
+    kept = kept[w[kept] >= np.longdouble(np.float32(min_p))]
+    return at[kept], w[kept]
