@@ -204,7 +204,8 @@ static __device__ __forceinline__ Scale scale_for(uint32_t top, double inv_t) {
     s.top = top;
     s.l_top = log_weight<OPACITY>(x);
     s.rate = inv_t * kLog2e;
-    s.unit = OPACITY && inv_t == 1.0 && x > -700.0;
+    // (further down, pow2's least value times this norm would be a weight: 2^-1000 e^300 is none, 2^-1000 e^690 is 0.04)
+    s.unit = OPACITY && inv_t == 1.0 && x > -300.0;
     s.norm = s.unit ? 1.0 + exp(-x) : 1.0;
     return s;
 }
