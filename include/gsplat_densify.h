@@ -157,8 +157,9 @@ size_t gs_relocate_workspace_bytes(int N, int pairs);
 /* Pair i makes row targets[i] a copy of row sources[i], in place.  A source with c pairs and its c copies become m = c + 1
  * Gaussians that together keep its opacity o and extent:  o' = 1 - (1 - o)^(1/m) (not below min_opacity),
  *   scales' = scales * o / sum_{j=1..m} (-1)^(j-1) C(m, j) o''^j / sqrt(j),   o'' = o' before the bound
- * (Kheradmand et al., 3D Gaussian Splatting as Markov Chain Monte Carlo, 2024); opacity logits above 16 count as 16.  Means,
- * quaternions and features are copied; the Adam moments of every row written (copies and sources) become 0.
+ * (Kheradmand et al., 3D Gaussian Splatting as Markov Chain Monte Carlo, 2024).  Opacity logits above 16 count as 16; where
+ * o is 0 these are the limits (scales as they are); a NaN logit makes logit and scales of the source and its copies NaN.
+ * Means, quaternions and features are copied; the Adam moments of every row written (copies and sources) become 0.
  *   params      the six tensors (K bases; features_rest NULL when K == 1)
  *   exp_avg, exp_avg_sq   nullable, as may be any of their tensors
  * Pairs that do not hold change nothing: an index outside [0, N) (gs_sample's -1 among them), a target that an earlier

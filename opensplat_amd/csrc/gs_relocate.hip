@@ -131,9 +131,20 @@ struct RelocateSets {
 
 constexpr int kRowPairs = 16;
 
-// log(o / D) and the new logit of a source with `m` equal shares; `inverse` [j] = {1 / j, 1 / sqrt(j)}
+// log(o / D) and the new logit of a source with `m` equal shares; `inverse` [j] = {1 / j, 1 / sqrt(j)}.
+// Below e^-40 what the sums differ by from their first terms is less than a rounding: o' = o / m, D = o, for logits whose
+// exponential is 0 too.  A NaN stays one (fmin and fmax would take the other operand).
 static __device__ __forceinline__ void share(float logit, int m, double min_logit, const double2 *inverse, float &new_logit,
                                              float &shrink) {
+    if (isnan(logit)) {
+        new_logit = shrink = logit;
+        return;
+    }
+    if (logit < -40.0f) {
+        new_logit = (float)fmax((double)logit - log((double)m), min_logit);
+        shrink = 0.0f;
+        return;
+    }
     const double x = fmin((double)logit, 16.0), z = log1p(exp(-fabs(x)));
     const double y = (fmax(x, 0.0) + z) / (double)m, p = -expm1(-y);   // softplus / m = -log(1 - o) / m
     double term = 1.0, sum = 0.0, left = (double)m * p;
