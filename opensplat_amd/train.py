@@ -25,6 +25,7 @@ optimiser-state surgery and the alpha reset, all on the device (include/gsplat_d
 """
 from __future__ import annotations
 
+import math
 import os
 
 import numpy as np
@@ -97,7 +98,7 @@ class Trainer:
         # (gs_relocate).  No statistics, no alpha reset.
         if strategy not in ("thresholds", "relocate"):
             raise ValueError("strategy must be 'thresholds' or 'relocate', not %r" % (strategy,))
-        if not 0.0 < min_opacity < 1.0 or not source_temperature > 0.0 or not 0.0 < source_top_p <= 1.0:
+        if not 0.0 < float(np.float32(min_opacity)) < 1.0 or not source_temperature > 0.0 or not 0.0 < source_top_p <= 1.0:
             raise ValueError("min_opacity in (0, 1), source_temperature > 0, source_top_p in (0, 1] needed")
         if strategy == "relocate" and reference_alpha_reset:
             raise ValueError("strategy='relocate' has no alpha reset")
@@ -759,7 +760,9 @@ class Trainer:
         """strategy="relocate": -> dict(relocated, added).  The draws come from the step number and the parameters alone:
         ranks with equal parameters take equal decisions.  One host synchronisation, to read how many are dead."""
         gen = torch.Generator(device=self.dev).manual_seed(1_000_003 * step)
-        logit = float(np.log(self.min_opacity / (1.0 - self.min_opacity)))
+        # the bound as gs_relocate forms and stores it, to the bit: of float32 min_opacity, rounded to float32
+        low = float(np.float32(self.min_opacity))
+        logit = float(np.float32(math.log(low / (1.0 - low))))
         dead = self.opacity_logits <= logit
         targets = dead.nonzero().view(-1).int()
         alive = self.N - targets.numel()
@@ -780,8 +783,9 @@ class Trainer:
                         a[old_n:].zero_()
                 setattr(self, name, new)
             self.N = old_n + grow
-            # (a row that found no source stays invisible until a later relocation)
-            self.params.v_opacity[old_n:] = logit
+            # (a row that finds no source, where all that is alive is NaN: far below what is rendered, a later relocation's)
+            self.params.v_opacity[old_n:] = min(logit, -20.0)
+            self.params.v_quats[old_n:, 0] = 1.0
             self._copy_sources(torch.arange(old_n, self.N, device=self.dev, dtype=torch.int32), sources, gen)
             self.grads = dist.GradBuffer(self.N, self.K, self.dev)
             self._shape = None               # per-N render buffers are rebuilt on the next render

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests.test_gpu_population import check_sample, dev, gaussian_set
+from tests.test_gpu_train_population import setup
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,38 @@ def test_relocate_does_not_hide_a_nan():
         assert np.array_equal(np.isnan(gpu[3].cpu().numpy().reshape(-1)), named)
         assert np.array_equal(np.isnan(gpu[1].cpu().numpy()).all(1), named)
         assert np.array_equal(gpu[0].cpu().numpy()[t], p[0][s])
+
+
+@pytest.mark.parametrize("min_opacity", [0.005, 0.02, 0.1])
+def test_growth_from_sources_that_the_copying_left_at_the_bound(min_opacity):
+    """One living Gaussian, just above the bound, takes all the others: every share stands at the bound, as gs_relocate
+    rounds it, and the set still grows by copies of it."""
+    T, cams, gts, bg = setup(N=500, strategy="relocate", refine_every=1, warmup_length=0, max_gaussians=600,
+                             min_opacity=min_opacity)
+    T.params.v_opacity[:] = -12.0
+    T.params.v_opacity[77] = float(np.log(min_opacity / (1 - min_opacity))) + 0.01
+    T.render(cams[0], bg, 1)
+    assert T.after_train(1) == dict(relocated=499, added=25) and T.N == 525
+    for t in (T.features_dc, T.features_rest, T.quats):
+        assert torch.equal(t[500:], t[77:78].expand_as(t[500:]))
+    # (each source's own copies share its extent: near the one that all come from, which nothing else is)
+    assert float((T.log_scales[500:] - T.log_scales[77]).abs().max()) < 0.1
+    assert (T.opacity_logits == T.opacity_logits[77]).all()
+
+
+def test_growth_without_a_source_adds_nothing_that_is_seen():
+    """All that is alive is NaN: no source can be drawn."""
+    T, cams, gts, bg = setup(N=400, strategy="relocate", refine_every=1, warmup_length=0, max_gaussians=500)
+    T.params.v_opacity[:] = -9.0
+    T.params.v_opacity[5] = float("nan")
+    T.render(cams[0], bg, 1)
+    assert T.after_train(1) == dict(relocated=399, added=20)
+    new = slice(400, 420)
+    assert (torch.sigmoid(T.opacity_logits[new]) < 1 / 255).all() and torch.isfinite(T.params.v_means[new]).all()
+    assert torch.equal(T.quats[new].norm(dim=1), torch.ones(20, device="cuda"))
+
+
+def test_bounds_that_are_none_in_float32_are_refused():
+    for low in (1.0 - 1e-9, 1e-60, float("nan")):
+        with pytest.raises(ValueError):
+            setup(N=50, strategy="relocate", min_opacity=low)
