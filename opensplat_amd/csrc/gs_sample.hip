@@ -1536,8 +1536,12 @@ static int launch_sample(const SampleArgs &a, const float *uniforms, int32_t *id
     if (L.chunks == 0) return launch_rows<DT, OPACITY>(a, uniforms, ids, s);
     const GsSampleConfig &c = a.cfg;
     const bool with_k = c.top_k_rows || c.top_k > 0, with_p = c.top_p_rows || c.top_p < 1.0f;
-    // a k that no list can hold, where the host knows it, and rows of more runs than a workgroup's table has go without
-    const bool lists = with_k && (c.top_k_rows || c.top_k <= kListMax) && a.cols <= (int64_t)kRunMax * kWaveEntries<DT>;
+    // Not for a k that no list can hold, where the host knows it, for rows of more runs than a workgroup's table has, or for
+    // more draws than one workgroup a row should make (1.4 us a thousand, where the whole chip makes a thousand draws of all
+    // the rows in 0.08; a list saves some 10 us of passes).  1 x 20000, top-k 4000: 4096 draws 45 us listed, 39 not, 32 768
+    // 82 and 40, 131 072 226 and 45; 16 x 1 M: 16 384 draws 81 and 97, 131 072 264 and 225; 64 x 131072: 32 768 119 and 218.
+    const bool lists = with_k && (c.top_k_rows || c.top_k <= kListMax) && a.cols <= (int64_t)kRunMax * kWaveEntries<DT> &&
+                       (int64_t)a.draws * (18 - a.rows) <= 18 * 4096;
     const LongArgs g = {(LongRow *)(ws + L.rows), (uint32_t *)(ws + L.k_count), (uint64_t *)(ws + L.p_mass),
                         (uint32_t *)(ws + L.p_count), (uint32_t *)(ws + L.chunk_max), (Mass *)(ws + L.chunk_sum),
                         (uint32_t *)(ws + L.chunk_ties), (Mass *)(ws + L.seg_sum), (Mass *)(ws + L.mid_sum),

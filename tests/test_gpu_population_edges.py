@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_population import check_sample, dev, gaussian_set
+from tests.test_gpu_population import check_sample, dev, gaussian_set, logits_of
 from tests.test_gpu_train_population import setup
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,15 @@ def test_bounds_that_are_none_in_float32_are_refused():
     for low in (1.0 - 1e-9, 1e-60, float("nan")):
         with pytest.raises(ValueError):
             setup(N=50, strategy="relocate", min_opacity=low)
+
+
+@pytest.mark.parametrize("rows,draws", [(1, 4336), (1, 4337), (2, 4608), (2, 4609), (2, 120_000), (17, 73_729), (20, 9000)])
+def test_sample_many_draws_behind_a_top_k_of_few(rows, draws):
+    """Long rows whose candidates fit a list, with few draws and with many: one workgroup's, or the whole chip's."""
+    rng = np.random.default_rng(draws)
+    x = logits_of(rng, rows, 20_000, "f32")
+    x[rows // 2] = -np.inf
+    x[rows // 2, 3_000:3_040] = 0.5
+    u = dev(rng.random((rows, draws), dtype=np.float32))
+    check_sample(x, u, top_k=700)
+    check_sample(x, u, top_k=dev(np.resize(np.array([30, 0, 4000], np.int32), rows)), temperature=0.7, top_p=0.8)
