@@ -221,7 +221,8 @@ void resetOpacity(torch::Tensor &opacities, float resetValue,
 //   relocateGaussians  rows `targets` become copies of rows `sources` (int32 [n]), in place; a source and its copies
 //                      together keep its opacity and extent; moments (may be empty) of the rows written become 0
 //   TileBalance        T sum_t (n_t / M) (S_t / S) of a frame's tile lists as an autograd node of the opacities (or
-//                      their logits) the records were packed from; returns a 0-dim tensor
+//                      their logits) the records were packed from; returns a 0-dim tensor.  Once differentiable in them:
+//                      a second derivative is refused
 torch::Tensor sampleIndices(const torch::Tensor &logits, const torch::Tensor &uniforms,
                             const c10::optional<torch::Tensor> &temperature = c10::nullopt,
                             const c10::optional<torch::Tensor> &topK = c10::nullopt,

@@ -996,13 +996,40 @@ Tensor TileBalance::forward(AutogradContext *ctx, Tensor opacities, Tensor packe
                                  fptr_mut(loss), nullptr, want ? fptr_mut(v) : nullptr,
                                  opacityIsLogit ? GS_FLAG_LOGIT_OPACITY : 0u, ws.data_ptr(), bytes, current_stream()),
                  "gs_tile_balance");
-    if (want) ctx->save_for_backward({v});
+    if (want) {
+        ctx->save_for_backward({v});
+        // (for their place in the graph alone: their values may change before the backward)
+        ctx->saved_data["opacities"] = opacities;
+    }
     return loss;
 }
 
+namespace {
+
+// The gradient as a node of its own, for backwards that are differentiated again: linear in the loss's cotangent; in the
+// opacities it is not formed, and a graph without that edge would take it for 0.
+class TileBalanceGrad : public torch::autograd::Function<TileBalanceGrad> {
+public:
+    static Tensor forward(AutogradContext *ctx, Tensor v, Tensor cotangent, Tensor /*opacities*/) {
+        ctx->save_for_backward({v});
+        return v * cotangent;
+    }
+    static tensor_list backward(AutogradContext *ctx, tensor_list grad_outputs) {
+        TORCH_CHECK(!ctx->needs_input_grad(2), "the tile balance loss cannot be differentiated twice with respect to the opacities");
+        return {Tensor(), (grad_outputs[0] * ctx->get_saved_variables()[0]).sum(), Tensor()};
+    }
+};
+
+}  // namespace
+
 tensor_list TileBalance::backward(AutogradContext *ctx, tensor_list grad_outputs) {
     const auto saved = ctx->get_saved_variables();
-    return {saved.empty() ? Tensor() : saved[0] * grad_outputs[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    Tensor grad;
+    if (!saved.empty())
+        grad = at::GradMode::is_enabled()
+                   ? TileBalanceGrad::apply(saved[0], grad_outputs[0], ctx->saved_data["opacities"].toTensor())
+                   : saved[0] * grad_outputs[0];
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
 }
 
 Tensor tileBalance(const Tensor &opacities, const BinnedLists &lists, bool opacityIsLogit) {

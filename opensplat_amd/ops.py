@@ -145,7 +145,7 @@ def sample_indices(logits, uniforms, temperature=None, top_k=None, top_p=None, m
 
 def tile_balance(opacities, packed, tile_bins, img_height, img_width, opacity_is_logit=False):
     """Balance loss of a frame's tile lists (gs_tile_balance) as an autograd node of the opacities (or logits) the
-    records `packed` were built from; returns a 0-dim tensor."""
+    records `packed` were built from; returns a 0-dim tensor (once differentiable: a second derivative is refused)."""
     return _ops.tile_balance(opacities, packed, tile_bins, int(img_height), int(img_width), bool(opacity_is_logit))
 
 

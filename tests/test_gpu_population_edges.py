@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+from opensplat_amd import cabi
 from tests.test_gpu_population import check_sample, dev, gaussian_set, logits_of
 from tests.test_gpu_train_population import setup
 
@@ -27,8 +28,6 @@ def test_sample_opacities_that_are_all_far_below(cols, top):
 @pytest.mark.parametrize("copies", [1, 2, 100])
 def test_relocate_sources_of_next_to_no_opacity(logit, copies):
     """o' = o / m and the extent stays, to 2^-54 of it for o below e^-37: logit' = x - log m, the scales as they are."""
-    from opensplat_amd import cabi
-
     rng = np.random.default_rng(copies)
     p, _, _ = gaussian_set(rng, copies + 3, 4, moments=False)
     p[3][1] = logit
@@ -43,8 +42,6 @@ def test_relocate_sources_of_next_to_no_opacity(logit, copies):
 
 def test_relocate_does_not_hide_a_nan():
     """A source whose logit is NaN: it and its copies get NaN logits and scales, no other row does."""
-    from opensplat_amd import cabi
-
     for pairs in (2, 3000):
         rng = np.random.default_rng(pairs)
         p, _, _ = gaussian_set(rng, 2 * pairs + 2, 1, moments=False)
@@ -105,3 +102,30 @@ def test_sample_many_draws_behind_a_top_k_of_few(rows, draws):
     u = dev(rng.random((rows, draws), dtype=np.float32))
     check_sample(x, u, top_k=700)
     check_sample(x, u, top_k=dev(np.resize(np.array([30, 0, 4000], np.int32), rows)), temperature=0.7, top_p=0.8)
+
+
+def test_second_derivative_of_the_balance_loss_is_refused():
+    """The gradient's own derivative with respect to the opacities is not formed: asking for it is an error, not 0.  With
+    respect to a factor of the loss it is the gradient."""
+    from opensplat_amd import ops
+    from tests.test_gpu_population import records
+
+    p, bins, _, _ = records(np.random.default_rng(1), 300, 200, 120)
+    packed, bins = torch.from_numpy(p).cuda(), torch.from_numpy(bins).cuda()
+    o = packed[:, 5].clone().requires_grad_(True)
+    f = torch.tensor(2.0, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(f * ops.tile_balance(o, packed, bins, 120, 200), o, create_graph=True)
+    want = cabi.tile_balance(200, 120, packed, bins)[2]
+    assert torch.equal(g.detach(), 2.0 * want)
+    d, = torch.autograd.grad(g.square().sum(), f, retain_graph=True)
+    assert abs(float(d) - 4.0 * float(want.double().square().sum())) <= 1e-5 * abs(float(d))
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(g.sum(), o, retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    # an optimiser's step between the forward and the backward, as before
+    loss = ops.tile_balance(o, packed, bins, 120, 200)
+    with torch.no_grad():
+        o.add_(1.0)
+    loss.backward()
+    assert torch.equal(o.grad, want)
