@@ -166,6 +166,13 @@ def _raw_stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _int32(what, *values):
+    """Refuses numbers that the C ABI's 32 bits do not hold: ctypes would pass their low halves."""
+    for v in values:
+        if not -0x80000000 <= v <= 0x7fffffff:
+            raise ValueError("%s: %d does not fit 32 bits" % (what, v))
+
+
 _ws_sizes = {}
 
 
@@ -725,6 +732,7 @@ def tile_balance(W, H, packed, tile_bins, scale=1.0, flags=0, want_grad=True, ou
             or not tile_bins.is_contiguous():
         raise ValueError("tile_bins must be contiguous int32 [%d, 2] on %s" % (tiles, dev))
     N = packed.shape[0]
+    _int32("tile_balance: image size and records", W, H, N)
     if out is None:
         if flags & GS_FLAG_ACCUMULATE_GRADS:
             raise ValueError("GS_FLAG_ACCUMULATE_GRADS adds to a v_opacity of the caller's: pass out")
@@ -880,6 +888,7 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
         raise ValueError("rows of the logits must not overlap")
     if uniforms.dtype != torch.float32 or uniforms.device != dev or not uniforms.is_contiguous():
         raise ValueError("uniforms must be contiguous float32 on %s" % dev)
+    _int32("sample: rows, entries and draws", R, V, shape[-1])
     cfg = GsSampleConfig(dtype, GS_FLAG_LOGIT_OPACITY if opacity else 0, 1.0, 0, 1.0, 0.0)
     for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if v is None:
@@ -891,6 +900,8 @@ def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=Non
                                  % (name, "int32" if name == "top_k" else "float32", R, dev))
             setattr(cfg, name + "_rows", v.data_ptr())
         else:
+            if name == "top_k":
+                _int32("sample: top_k", v)
             setattr(cfg, name, v)
     if out is None:
         out = torch.empty(shape, device=dev, dtype=torch.int32)
@@ -933,6 +944,7 @@ def relocate(params, exp_avg, exp_avg_sq, targets, sources, min_opacity=0.005, w
                                  "on %s" % (N, K, lens, dev))
             at[i] = t.data_ptr() if lens[i] else 0
         sets.append(C.byref(GsGaussianSet(*at)))
+    _int32("relocate: rows, bases and pairs", N, K, n)
     if N == 0 or n == 0:
         return
     with _on(dev):

@@ -983,6 +983,8 @@ Tensor TileBalance::forward(AutogradContext *ctx, Tensor opacities, Tensor packe
     GS_CHECK_F32(opacities); GS_CHECK_F32(packed); GS_CHECK_I32(tileBins);
     const int64_t N = packed.size(0), tiles = ((imgWidth + 15) / 16) * ((imgHeight + 15) / 16);
     TORCH_CHECK(packed.dim() == 2 && packed.size(1) == GS_SPLAT_DWORDS && packed.is_contiguous(), "packed must be [N, 12]");
+    TORCH_CHECK(N <= INT32_MAX && imgWidth > 0 && imgHeight > 0 && imgWidth <= INT32_MAX && imgHeight <= INT32_MAX,
+                "at most 2^31 - 1 records and an image size expected");
     TORCH_CHECK(tileBins.numel() == 2 * tiles && tileBins.is_contiguous(), "tileBins must be [tiles, 2]");
     TORCH_CHECK(opacities.numel() == N, "one opacity per record");
     TORCH_CHECK(packed.device() == opacities.device() && tileBins.device() == opacities.device(), "one device expected");

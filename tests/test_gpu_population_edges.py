@@ -129,3 +129,27 @@ def test_second_derivative_of_the_balance_loss_is_refused():
         o.add_(1.0)
     loss.backward()
     assert torch.equal(o.grad, want)
+
+
+def test_numbers_that_do_not_fit_the_c_abi_are_refused():
+    """32-bit sizes and settings: a larger one is an error, not its low half."""
+    x, u = torch.zeros((1, 20), device="cuda"), torch.rand((1, 8), device="cuda")
+    for k in (2 ** 31, 2 ** 32 + 1, -2 ** 31 - 1):
+        with pytest.raises(ValueError):
+            cabi.sample(x, u, top_k=k)
+    assert cabi.sample(x, u, top_k=2 ** 31 - 1).shape == (1, 8)
+    wide = torch.empty(2 ** 32 + 5, device="cuda", dtype=torch.float16)
+    with pytest.raises(ValueError):
+        cabi.sample(wide, u[0])
+    del wide
+    many = torch.empty(2 ** 32, device="cuda", dtype=torch.float32)
+    with pytest.raises(ValueError):
+        cabi.sample(x[0], many)
+    with pytest.raises(ValueError):
+        cabi.sample(many.view(-1, 1), many.view(-1, 1))
+    i = many.view(torch.int32)
+    p = [torch.zeros(s, device="cuda") for s in ((9, 3), (9, 3), (9, 4), (9, 1), (9, 3))] + [None]
+    with pytest.raises(ValueError):
+        cabi.relocate(p, None, None, i, i)
+    del many, i
+    torch.cuda.empty_cache()
