@@ -49,19 +49,30 @@ def _run(cmd: list[str]) -> None:
     subprocess.check_call(cmd, cwd=CSRC)
 
 
+def _compile_hip(target: str, extra: list[str], tag: str = "") -> None:
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    objects = []
+    for s in HIP_SOURCES_PLAIN:
+        objects.append(s.replace(".hip", tag + ".o"))
+        flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+        _run([hipcc] + flags + HIPCC_PLAIN_FLAGS + extra + ["-c", s, "-o", objects[-1]])
+    # (objects first: a source file name makes hipcc read everything behind it as source)
+    _run([hipcc] + HIPCC_FLAGS + extra + objects + HIP_SOURCES + ["-o", target])
+
+
 def build_hip(force: bool = False) -> str:
     srcs = [os.path.join(CSRC, s) for s in HIP_SOURCES + HIP_SOURCES_PLAIN]
     deps = srcs + [h if os.path.isabs(h) else os.path.join(CSRC, h) for h in HIP_HEADERS]
     if force or _stale(HIP_LIB, deps):
-        hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-        objects = []
-        for s in HIP_SOURCES_PLAIN:
-            objects.append(s.replace(".hip", ".o"))
-            flags = [f for f in HIPCC_FLAGS if f != "-shared"]
-            _run([hipcc] + flags + HIPCC_PLAIN_FLAGS + ["-c", s, "-o", objects[-1]])
-        # (objects first: a source file name makes hipcc read everything behind it as source)
-        _run([hipcc] + HIPCC_FLAGS + objects + HIP_SOURCES + ["-o", HIP_LIB])
+        _compile_hip(HIP_LIB, [])
     return HIP_LIB
+
+
+def build_variant(name: str, extra: list[str]) -> str:
+    """libgsplat_hip_<name>.so: the same sources with further hipcc flags (scripts/build_variant.sh)."""
+    target = os.path.join(CSRC, "libgsplat_hip_%s.so" % name)
+    _compile_hip(target, list(extra), "_" + name)
+    return target
 
 
 def build_torch(force: bool = False) -> str:
