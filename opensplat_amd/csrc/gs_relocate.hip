@@ -79,49 +79,40 @@ k_relocate_count(int N, int pairs, const int32_t *__restrict__ targets, const in
     out[i] = p;
 }
 
-// The three of them for few pairs, as one workgroup's phases (launches of a microsecond of work cost the host two each).
+// The three of them for few pairs, as one workgroup's phases, a pair a thread (launches of a microsecond of work cost the host
+// two each).  Its one compute unit's loads and atomics grow with the pairs: calls of 300 pairs 15.6 us against 21.5 in three
+// launches, 640 17.8 and 21.6, 1000 22.9 and 21.8 (2000, two pairs a thread, 38 and 22).
 // The words pass through the device's atomics: a load of this unit's own cache could be older.
-constexpr int kFewPairs = 2048;
-__global__ void __launch_bounds__(1024)
+constexpr int kFewPairs = 768;
+__global__ void __launch_bounds__(kFewPairs)
 k_relocate_few(int N, int pairs, const int32_t *__restrict__ targets, const int32_t *__restrict__ sources, int32_t *owner,
                int32_t *copies, const float *__restrict__ logits, const float *__restrict__ log_scales,
                RelocatePair *__restrict__ out) {
-    int32_t t[kFewPairs / 1024], s[kFewPairs / 1024];
-#pragma unroll
-    for (int k = 0; k < kFewPairs / 1024; k++) {
-        const int i = k * 1024 + threadIdx.x;
-        t[k] = s[k] = -1;
-        if (i < pairs) {
-            t[k] = targets[i];
-            s[k] = sources[i];
-        }
-        if (in_range(t[k], N) && in_range(s[k], N)) {
-            __hip_atomic_store(&owner[t[k]], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&owner[s[k]], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&copies[s[k]], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        } else {
-            t[k] = -1;
-        }
+    const int i = threadIdx.x;
+    int32_t t = -1, s = -1;
+    if (i < pairs) {
+        t = targets[i];
+        s = sources[i];
+    }
+    const bool valid = in_range(t, N) && in_range(s, N);
+    if (valid) {
+        __hip_atomic_store(&owner[t], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&owner[s], kNoOwner, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&copies[s], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kFewPairs / 1024; k++)
-        if (t[k] >= 0) atomicMin(&owner[t[k]], k * 1024 + (int)threadIdx.x);
+    if (valid) atomicMin(&owner[t], i);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kFewPairs / 1024; k++) {
-        const int i = k * 1024 + threadIdx.x;
-        RelocatePair p = {0.0f, 0.0f, 0.0f, 0.0f, -1};
-        if (t[k] >= 0 && __hip_atomic_load(&owner[t[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i &&
-            __hip_atomic_load(&owner[s[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kNoOwner) {
-            p.logit = logits[s[k]];
-            p.s0 = log_scales[3 * (size_t)s[k]];
-            p.s1 = log_scales[3 * (size_t)s[k] + 1];
-            p.s2 = log_scales[3 * (size_t)s[k] + 2];
-            p.rank = atomicAdd(&copies[s[k]], 1);
-        }
-        if (i < pairs) out[i] = p;
+    RelocatePair p = {0.0f, 0.0f, 0.0f, 0.0f, -1};
+    if (valid && __hip_atomic_load(&owner[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i &&
+        __hip_atomic_load(&owner[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kNoOwner) {
+        p.logit = logits[s];
+        p.s0 = log_scales[3 * (size_t)s];
+        p.s1 = log_scales[3 * (size_t)s + 1];
+        p.s2 = log_scales[3 * (size_t)s + 2];
+        p.rank = atomicAdd(&copies[s], 1);
     }
+    if (i < pairs) out[i] = p;
 }
 
 struct RelocateSets {
@@ -270,7 +261,7 @@ extern "C" int gs_relocate(int N, int K, int pairs, const int32_t *targets, cons
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid((pairs + kRelThreads - 1) / kRelThreads), block(kRelThreads);
     if (pairs <= kFewPairs) {
-        GS_LAUNCH(k_relocate_few, dim3(1), dim3(1024), 0, s, N, pairs, targets, sources, owner, copies, p.opacity_logits,
+        GS_LAUNCH(k_relocate_few, dim3(1), dim3(kFewPairs), 0, s, N, pairs, targets, sources, owner, copies, p.opacity_logits,
                   p.log_scales, held);
         GS_LAUNCH_CHECK();
     } else {

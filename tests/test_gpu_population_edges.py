@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from opensplat_amd import cabi
-from tests.test_gpu_population import check_sample, dev, gaussian_set, logits_of
+from tests.test_gpu_population import check_relocate, check_sample, dev, gaussian_set, logits_of
 from tests.test_gpu_train_population import setup
 
 pytestmark = pytest.mark.gpu
@@ -153,3 +153,14 @@ def test_numbers_that_do_not_fit_the_c_abi_are_refused():
         cabi.relocate(p, None, None, i, i)
     del many, i
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [511, 512, 513, 767, 768, 769, 1023, 1025, 2047, 2049])
+def test_relocate_around_the_launch_forms(n):
+    """One workgroup's phases and three launches give the same; among the pairs some that do not hold."""
+    rng = np.random.default_rng(n)
+    N = 3 * n
+    order = rng.permutation(N)
+    targets, sources = order[:n].astype(np.int64), order[n:][(rng.random(n) ** 3 * n).astype(int)]
+    targets[5], targets[n - 1], sources[7], sources[n // 2] = targets[n - 2], -1, targets[3], N
+    check_relocate(gaussian_set(rng, N, 4), targets.tolist(), sources.tolist())
