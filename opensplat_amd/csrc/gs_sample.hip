@@ -1403,7 +1403,9 @@ k_long_draw(SampleArgs a, LongArgs g, int blocks, const float *__restrict__ unif
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-constexpr int kRowLimit = 8192;                // longest row of the one-workgroup form
+// Longest row of the one-workgroup form, what 1024 threads hold in registers.  Calls of 8192 entries with top-p, so / in the
+// longer rows' launches: 1 row 13.5 / 39 us, 256 rows 14.2 / 56, 1024 rows 52 / 148; with nothing cut 9.0 / 15.6 and 28 / 31.
+constexpr int kRowLimit = 8192;
 
 struct SampleLayout {
     size_t rows, k_count, p_mass, p_count, chunk_max, chunk_sum, chunk_ties, seg_sum, mid_sum, top_sum, seg_ties, list, list_index,
@@ -1448,11 +1450,13 @@ static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids,
     return GS_OK;
 }
 
-// Up to this many chunks (16 M entries) the launch behind k_long_max reads the chunks' maxima itself, a few loads a thread;
-// beyond, that would grow with the square of the row.
-constexpr int kOwnMaxChunks = 4096;
+// Up to this many chunks (8 M entries) the launch behind k_long_max reads the chunks' maxima itself, a few loads a thread;
+// beyond, that would grow with the square of the row.  Rows with nothing cut, in a launch of its own / in the next one:
+// 1 M 22.2 / 18.7 us a call, 5 M 29.6 / 28.3, 16 M 56 / 62, 40 M 113 / 140.
+constexpr int kOwnMaxChunks = 2048;
 
-// Up to this many draws a wave each, in fewer steps: 64 draws of 64 rows 4.0 us, a thread each 10.
+// Up to this many draws a wave each, in fewer steps and without a scan's launch for short rows.  Calls of 64 x 131072 with
+// nothing cut, a wave / eight lanes a draw: 64 draws 30.4 / 33.3 us, 2048 31.1 / 33.4, 16 384 37.4 / 34.5.
 constexpr int64_t kWaveDraws = 2048;
 
 template <int DT, bool OPACITY, bool CUT>
