@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from opensplat_amd import cabi
-from tests.test_gpu_population import check_relocate, check_sample, dev, gaussian_set, logits_of
+from tests.test_gpu_population import check_relocate, check_sample, dev, gaussian_set, logits_of, records
 from tests.test_gpu_train_population import setup
 
 pytestmark = pytest.mark.gpu
@@ -108,7 +108,6 @@ def test_second_derivative_of_the_balance_loss_is_refused():
     """The gradient's own derivative with respect to the opacities is not formed: asking for it is an error, not 0.  With
     respect to a factor of the loss it is the gradient."""
     from opensplat_amd import ops
-    from tests.test_gpu_population import records
 
     p, bins, _, _ = records(np.random.default_rng(1), 300, 200, 120)
     packed, bins = torch.from_numpy(p).cuda(), torch.from_numpy(bins).cuda()
@@ -164,3 +163,90 @@ def test_relocate_around_the_launch_forms(n):
     targets, sources = order[:n].astype(np.int64), order[n:][(rng.random(n) ** 3 * n).astype(int)]
     targets[5], targets[n - 1], sources[7], sources[n // 2] = targets[n - 2], -1, targets[3], N
     check_relocate(gaussian_set(rng, N, 4), targets.tolist(), sources.tolist())
+
+
+def test_tile_balance_of_a_4k_frame_captured():
+    """A table that takes most of the LDS, asked for inside a capture; replayed with eager calls between."""
+    p, bins, lists, _ = records(np.random.default_rng(0), 4000, 3840, 2160)
+    packed, bins = dev(p), dev(bins)
+    want = [t.clone() for t in cabi.tile_balance(3840, 2160, packed, bins)]
+    assert np.array_equal(want[1].cpu().numpy(), lists)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        out = cabi.tile_balance(3840, 2160, packed, bins)
+    for turn in range(4):
+        for t in out:
+            t.zero_()
+        packed[:, 5] = packed[:, 5].roll(turn)
+        want = [t.clone() for t in cabi.tile_balance(3840, 2160, packed, bins)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
+def test_balance_through_the_factored_exchange():
+    """The opacities' gradient is the flat exchange's to the bit; one camera and a batch."""
+    grads = []
+    for exchange in ("flat", "factored"):
+        T, cams, gts, bg = setup(balance_weight=0.4, deterministic=True, exchange=exchange)
+        T.factored = exchange == "factored"
+        T.train_step(cams[0], gts[0], bg, 1)
+        one = T.grads.v_opacity.clone()
+        T2, _, _, _ = setup(balance_weight=0.4, deterministic=True, exchange=exchange)
+        T2.train_step_batch(cams, gts, bg, 1, step_optimizer=False)
+        torch.cuda.synchronize()
+        grads.append((one, T2.grads.v_opacity.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*grads)) and (grads[0][0] != 0).any()
+
+
+@pytest.mark.parametrize("K", [1, 9])
+def test_a_budget_with_other_numbers_of_bases(K):
+    T, cams, gts, bg = setup(N=1500, K=K, strategy="relocate", refine_every=2, warmup_length=0, max_gaussians=1700,
+                             balance_weight=0.01)
+    for step in range(1, 9):
+        T.params.v_opacity[step::50] = -8.0
+        T.train_step_batch(cams, gts, bg, 0 if K == 1 else 1, step=step)
+        c = T.after_train(step)
+        assert (c is None) == (step % 2 == 1)
+    assert T.N == 1700 and all(torch.isfinite(t).all() for t in T._param_list(T.params) if t is not None)
+
+
+def test_sample_in_a_workspace_of_the_callers():
+    """One workspace for calls of other shapes, in stream order; one byte less is refused, as is one at an odd address."""
+    rng = np.random.default_rng(3)
+    need = max(cabi.lib().gs_sample_workspace_bytes(r, c) for r, c in ((3, 20_000), (1, 70_000), (5, 900)))
+    ws = torch.full((need + 64,), 0xA5, device="cuda", dtype=torch.uint8)
+    for r, c in ((3, 20_000), (1, 70_000), (5, 900), (3, 20_000)):
+        x, u = logits_of(rng, r, c, "f32"), dev(rng.random((r, 20), dtype=np.float32))
+        for kw in (dict(), dict(top_k=30, top_p=0.7), dict(top_p=0.7), dict(top_k=9000)):
+            got = cabi.sample(x, u, workspace=ws[:need], **kw)
+            assert torch.equal(got, cabi.sample(x, u, **kw))
+            assert (ws[need:] == 0xA5).all()
+    x, u = logits_of(rng, 1, 70_000, "f32"), dev(rng.random((1, 20), dtype=np.float32))
+    with pytest.raises(ValueError):
+        cabi.sample(x, u, workspace=ws[:cabi.lib().gs_sample_workspace_bytes(1, 70_000) - 1])
+    with pytest.raises(RuntimeError):
+        cabi.sample(x, u, workspace=ws[8:])
+
+
+def test_sample_a_row_of_two_thousand_million():
+    """Indices, chunks and places of a row that ends shortly before 2^31 entries."""
+    n = 2_000_000_011
+    x = torch.full((n,), -torch.inf, device="cuda", dtype=torch.float16)
+    at = torch.tensor([7, 4096, 1_073_741_823, 1_073_741_824, 1_999_999_999, n - 1])
+    x[at.cuda()] = torch.tensor([0.0, 1.0, 1.0, -1.0, 2.0, 1.0], dtype=torch.float16).cuda()
+    u = torch.linspace(0, 1 - 2.0 ** -24, 301)
+    w = torch.exp(x[at.cuda()].double().cpu() - 2.0)
+
+    def want(keep):
+        mass = (w * keep).cumsum(0)
+        return at[torch.searchsorted(mass, u.double() * mass[-1], right=True)].int()
+
+    every = torch.ones(6)
+    for kw, keep in ((dict(), every), (dict(top_k=3), torch.tensor([0, 1, 1, 0, 1, 0])), (dict(min_p=0.2), w >= 0.2),
+                     (dict(top_p=0.5), torch.tensor([0, 1, 0, 0, 1, 0]))):
+        assert torch.equal(cabi.sample(x, u.cuda(), **kw).cpu(), want(keep)), kw
+    del x
+    torch.cuda.empty_cache()
