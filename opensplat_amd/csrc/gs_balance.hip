@@ -64,7 +64,7 @@ k_balance_rows(BalanceGrid g, const int2 *__restrict__ bins, int32_t *__restrict
     }
 }
 
-// Down the columns; four threads a column would share it in LDS (below), here the rows' loads are simply under way together.
+// Down the columns, a thread each, eight rows' loads under way together.
 __global__ void __launch_bounds__(64)
 k_balance_cols(BalanceGrid g, int32_t *__restrict__ table) {
     const int x = blockIdx.x * 64 + threadIdx.x;
@@ -109,18 +109,6 @@ static __device__ __forceinline__ double block_sum_f64(double v, double *red /* 
     return r;
 }
 
-// Inclusive sum over the wave's lanes without LDS: shifts by 1, 2, 4, 8 inside rows of 16, then each row's last lane into
-// the next row, then lane 31 into the upper half.
-static __device__ __forceinline__ int32_t wave_scan(int32_t v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 constexpr int kSumThreads = 1024;
 constexpr int kSumParts = 256;                 // workgroups at most: one per compute unit
 constexpr int kColParts = 4;
@@ -158,7 +146,7 @@ static __device__ __forceinline__ void lds_table(const BalanceGrid &g, const int
         int32_t base = 0;
         for (int x0 = 1; x0 <= g.tw; x0 += 64) {
             const int x = x0 + lane;
-            const int32_t s = wave_scan(x <= g.tw ? table[y * g.pitch + x] : 0);
+            const int32_t s = (int32_t)wave_scan((uint32_t)(x <= g.tw ? table[y * g.pitch + x] : 0));
             if (x <= g.tw) table[y * g.pitch + x] = base + s;
             base += __builtin_amdgcn_readlane(s, 63);
         }

@@ -95,6 +95,37 @@ __device__ __forceinline__ int wave_max_i(int v) {
     return max(max(s0, s1), max(s2, s3));
 }
 
+// Inclusive sum over the wave's lanes without LDS: shifts by 1, 2, 4, 8 inside rows of 16, then each row's last lane into
+// the next row, then lane 31 into the upper half.  Words of one, two or four registers.
+using uint128 = unsigned __int128;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+    return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint128 from_lane(uint128 v) {
+    return (uint128)from_lane<CTRL, ROWS>((uint64_t)v) | (uint128)from_lane<CTRL, ROWS>((uint64_t)(v >> 64)) << 64;
+}
+template <typename T>
+__device__ __forceinline__ T row_scan(T v) {   // (the steps inside rows of 16)
+    v += from_lane<0x111, 0xF>(v);
+    v += from_lane<0x112, 0xF>(v);
+    v += from_lane<0x114, 0xF>(v);
+    v += from_lane<0x118, 0xF>(v);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
+    v += from_lane<0x142, 0xA>(v);
+    v += from_lane<0x143, 0xC>(v);
+    return v;
+}
+
 // ---- glibc-compatible expf ------------------------------------------------------------------
 // Table of 2^(i/32) (bits, minus i<<47) and polynomial of the expf that glibc >= 2.27 ships
 // (sysdeps/ieee754/flt-32/e_expf.c, N = 32, computed in double).  Checked exhaustively against

@@ -246,7 +246,7 @@ struct SearchOf {
 using Search = SearchOf<uint64_t, double>;
 
 // Masses of the longer rows, in units of 1 / high^2.
-using Mass = unsigned __int128;
+using Mass = uint128;
 using MassSearch = SearchOf<Mass, Mass>;
 
 // A weight as high * hi + lo, |lo| <= high / 2: sums of either word over a row stay below 2^63, without carries.
@@ -286,20 +286,6 @@ static __device__ __forceinline__ uint64_t fixed(double w, double unit) {
     return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) - 0x4330000000000000ull;
 }
 
-// Inclusive sum over the wave's lanes without LDS: shifts by 1, 2, 4, 8 inside rows of 16, then each row's last lane into
-// the next row, then lane 31 into the upper half.
-template <int CTRL, int ROWS>
-static __device__ __forceinline__ uint32_t from_lane(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF);
-}
-template <int CTRL, int ROWS>
-static __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
-    return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
-}
-template <int CTRL, int ROWS>
-static __device__ __forceinline__ Mass from_lane(Mass v) {
-    return (Mass)from_lane<CTRL, ROWS>((uint64_t)v) | (Mass)from_lane<CTRL, ROWS>((uint64_t)(v >> 64)) << 64;
-}
 // A lane's value as one that the wave has in common, in scalar registers: `lane` is in common too.
 static __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
@@ -312,21 +298,6 @@ static __device__ __forceinline__ Mass lane_value(Mass v, int lane) {
 }
 static __device__ __forceinline__ Mass shuffle(Mass v, int lane) {
     return (Mass)__shfl((uint64_t)v, lane, 64) | (Mass)__shfl((uint64_t)(v >> 64), lane, 64) << 64;
-}
-template <typename T>
-static __device__ __forceinline__ T row_scan(T v) {   // (the steps inside rows of 16)
-    v += from_lane<0x111, 0xF>(v);
-    v += from_lane<0x112, 0xF>(v);
-    v += from_lane<0x114, 0xF>(v);
-    v += from_lane<0x118, 0xF>(v);
-    return v;
-}
-template <typename T>
-static __device__ __forceinline__ T wave_scan(T v) {
-    v = row_scan(v);
-    v += from_lane<0x142, 0xA>(v);
-    v += from_lane<0x143, 0xC>(v);
-    return v;
 }
 
 // Exclusive scan over the workgroup in thread order, THREADS a multiple of 64 up to 1024; `total` gets the sum.  Each wave
