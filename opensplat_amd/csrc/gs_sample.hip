@@ -408,11 +408,12 @@ struct RowShared {
 };
 
 // A row's selection and its draws, by one workgroup; thread t holds the keys of entries 8 t .. 8 t + 7, so that thread order
-// is index order.  `mx`: the largest key, not 0.  `f_k`: the search of top-k as it stands before digit `level_k`.  `index(i)`: the index in the row of entry i.
+// is index order.  `mx`: the largest key, not 0.  `f_k`: the search of top-k as it stands before digit `level_k`.  Of the
+// draws, those of `part` of `parts`.  `index(i)`: the index in the row of entry i.
 template <int DT, bool OPACITY, int THREADS, typename F>
 static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSettings &set, int r, const uint32_t (&key)[kEach],
-                                                uint32_t mx, Search f_k, int level_k, RowShared<THREADS> &sh,
-                                                const float *__restrict__ uniforms,
+                                                uint32_t mx, Search f_k, int level_k, int part, int parts,
+                                                RowShared<THREADS> &sh, const float *__restrict__ uniforms,
                                                 int32_t *__restrict__ ids, F index) {
     constexpr bool kSplit = RowShared<THREADS>::kSplit;
     constexpr int kPitch = RowShared<THREADS>::kPitch, kRowCopies = RowShared<THREADS>::kCopies;
@@ -534,7 +535,7 @@ static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSe
     uint64_t total;
     run_sum[tid] = block_scan<THREADS>(sum, waves_u, total);
     __syncthreads();
-    for (int j = tid; j < a.draws; j += THREADS) {
+    for (int64_t j = (int64_t)part * THREADS + tid; j < a.draws; j += (int64_t)parts * THREADS) {
         const float u = uniforms[(size_t)r * a.draws + j];
         const uint64_t goal = set.greedy ? 0ull : goal_of(u, total);
         int lo = 0, hi = THREADS;              // run_sum[lo] <= goal < run_sum[hi]
@@ -551,13 +552,13 @@ static __device__ __forceinline__ void draw_row(const SampleArgs &a, const RowSe
     }
 }
 
-// One workgroup per row.  Bound by latency: a dozen barriers, and per digit one LDS atomic an entry; the entries are read
-// once.
+// `parts` workgroups per row, each with a share of its draws; the selection is each one's own.  Bound by latency: a dozen
+// barriers, and per digit one LDS atomic an entry; the entries are read once.
 template <int DT, bool OPACITY, int THREADS>
 __global__ void __launch_bounds__(THREADS)
-k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
+k_sample_row(SampleArgs a, int parts, const float *__restrict__ uniforms, int32_t *__restrict__ ids) {
     __shared__ RowShared<THREADS> sh;
-    const int r = blockIdx.x, tid = threadIdx.x, n = a.cols;
+    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x, n = a.cols;
     const char *row = static_cast<const char *>(a.logits) + (size_t)r * a.stride * kBytes<DT>;
     const RowSettings set = row_settings(a, r);
     uint32_t key[kEach];
@@ -579,10 +580,11 @@ k_sample_row(SampleArgs a, const float *__restrict__ uniforms, int32_t *__restri
         for (int w = 0; w < THREADS / 64; w++) mx = max(mx, sh.waves_i[w]);
     }
     if (!set.ok || mx == 0) {
-        for (int j = tid; j < a.draws; j += THREADS) ids[(size_t)r * a.draws + j] = -1;
+        for (int64_t j = (int64_t)part * THREADS + tid; j < a.draws; j += (int64_t)parts * THREADS)
+            ids[(size_t)r * a.draws + j] = -1;
         return;
     }
-    draw_row<DT, OPACITY, THREADS>(a, set, r, key, mx, {0, (double)set.top_k, 0, 0}, 0, sh, uniforms, ids,
+    draw_row<DT, OPACITY, THREADS>(a, set, r, key, mx, {0, (double)set.top_k, 0, 0}, 0, part, parts, sh, uniforms, ids,
                                    [](int i) { return i; });
 }
 
@@ -1062,7 +1064,8 @@ k_long_list(SampleArgs a, LongArgs g, const float *__restrict__ uniforms, int32_
 #pragma unroll
     for (int e = 0; e < kEach; e++) key[e] = keys[tid * kEach + e];
     __syncthreads();
-    draw_row<DT, OPACITY, kListThreads>(a, row_settings(a, r), r, key, st.scale.top, st.k[0], 1, sh, uniforms, ids,
+    draw_row<DT, OPACITY, kListThreads>(a, row_settings(a, r), r, key, st.scale.top, st.k[0], 1, 0, 1, sh, uniforms,
+                                        ids,
                                         [&](int i) { return order[i]; });
 }
 
@@ -1407,18 +1410,24 @@ struct SampleLayout {
     }
 };
 
-template <int DT, bool OPACITY>
-static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids, hipStream_t s) {
-    const dim3 grid(a.rows);
-    if (a.cols <= 64 * kEach) {
-        GS_LAUNCH((k_sample_row<DT, OPACITY, 64>), grid, dim3(64), 0, s, a, uniforms, ids);
-    } else if (a.cols <= 256 * kEach) {
-        GS_LAUNCH((k_sample_row<DT, OPACITY, 256>), grid, dim3(256), 0, s, a, uniforms, ids);
-    } else {
-        GS_LAUNCH((k_sample_row<DT, OPACITY, 1024>), grid, dim3(1024), 0, s, a, uniforms, ids);
-    }
+// Eight draws a thread pay for a selection of one's own, as long as all the workgroups are resident at once.  With top-p, one
+// workgroup a row / so: 1 x 8160, 16 384 draws 40 / 27 us, 1 M 1742 / 29; 1 x 28, 1024 draws 32 / 26, 100 000 1316 / 27;
+// 2000 x 28 (more rows than are resident) would go from 111 to 198 with two a row.
+template <int DT, bool OPACITY, int THREADS>
+static int launch_row_form(const SampleArgs &a, const float *uniforms, int32_t *ids, hipStream_t s) {
+    const int64_t room = 256 * (160 * 1024 / (int64_t)sizeof(RowShared<THREADS>)) / a.rows, share = 8 * THREADS;
+    int64_t parts = ((int64_t)a.draws + share - 1) / share;
+    parts = parts < room ? parts : (room < 1 ? 1 : room);
+    GS_LAUNCH((k_sample_row<DT, OPACITY, THREADS>), dim3((unsigned)(parts * a.rows)), dim3(THREADS), 0, s, a, (int)parts, uniforms,
+              ids);
     GS_LAUNCH_CHECK();
     return GS_OK;
+}
+template <int DT, bool OPACITY>
+static int launch_rows(const SampleArgs &a, const float *uniforms, int32_t *ids, hipStream_t s) {
+    if (a.cols <= 64 * kEach) return launch_row_form<DT, OPACITY, 64>(a, uniforms, ids, s);
+    if (a.cols <= 256 * kEach) return launch_row_form<DT, OPACITY, 256>(a, uniforms, ids, s);
+    return launch_row_form<DT, OPACITY, 1024>(a, uniforms, ids, s);
 }
 
 // Up to this many chunks (8 M entries) the launch behind k_long_max reads the chunks' maxima itself, a few loads a thread;

@@ -250,3 +250,18 @@ def test_sample_a_row_of_two_thousand_million():
         assert torch.equal(cabi.sample(x, u.cuda(), **kw).cpu(), want(keep)), kw
     del x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(1, 28, 512), (1, 28, 513), (1, 400, 70_000), (3, 1500, 2049), (2, 8192, 8193),
+                                   (1, 8160, 100_001), (600, 2100, 9000), (9000, 10, 600)])
+def test_sample_many_draws_of_short_rows(shape):
+    """A row's draws shared by several workgroups; where the rows fill the chip, by one each."""
+    rows, cols, draws = shape
+    rng = np.random.default_rng(draws)
+    x = logits_of(rng, rows, cols, "f32", pad=1)
+    x[rows // 2, cols // 2:] = -np.inf
+    if rows > 2:
+        x[1] = np.nan
+    u = dev(rng.random((rows, draws), dtype=np.float32))
+    # (the temperature as the call takes it: of five million draws, some lie closer to a border than 0.8 to its float32)
+    check_sample(x, u, temperature=float(np.float32(0.8)), top_p=0.9)
