@@ -146,9 +146,9 @@ size_t gs_sample_workspace_bytes(int rows, int cols);
  *               -1 for a row without candidates and for a NaN uniform
  * logits [rows, cols] of `dtype`, row r at row_stride elements behind row r - 1 (row_stride >= cols; any alignment of the
  * element); uniforms and ids [rows, draws] contiguous.  Weights are 64-bit, relative to the row's largest, and rounded
- * once: to multiples of 2^-50 (2^-49 beyond 4096 entries) in rows of up to 8192 entries, and in longer ones that top-k
- * cuts to as few; to multiples of 2^-(124 - 2 ceil log2 cols) in all other rows.  One that rounds to 0 is never drawn.
- * Their sums are exact: equal calls give equal ids.  No host synchronisation; the workspace (16-byte aligned) may be reused behind the call in stream order. */
+ * once: to multiples of 2^-50 (2^-49 beyond 4096 entries) in rows of up to 8192 entries, at least as finely in longer ones
+ * that top-k cuts to as few, to multiples of 2^-(124 - 2 ceil log2 cols) in all other rows.  One that rounds to 0 is never
+ * drawn.  Their sums are exact: equal calls give equal ids.  No host synchronisation; the workspace (16-byte aligned) may be reused behind the call in stream order. */
 int gs_sample(int rows, int cols, const void *logits, int64_t row_stride, const GsSampleConfig *cfg /*host*/, int draws,
               const float *uniforms, int32_t *ids, void *workspace, size_t workspace_bytes, gs_stream_t stream);
 

@@ -13,6 +13,7 @@
 //   k_relocate_claim   a target belongs to the first pair that names it; every target of a pair in range is marked
 //   k_relocate_count   pairs that hold (own target, source that is no target) are counted per source; the pair that is
 //                      counted first also rewrites the source — which one that is changes no result
+//   k_relocate_few     these three, where pairs are few
 //   k_relocate_rows    16 pairs per workgroup: one lane each for opacity and extent, then their rows, a wave for four pairs
 //                      with a lane per column of the six tensors, so that a row is one load and its copy one store
 // A source's opacity and scales are rewritten by one workgroup while others may hold pairs of the same source: those
@@ -20,8 +21,9 @@
 // stay as they are.
 //
 // Bound by scattered lines: a row of 59 floats lies in six places (some nine 64-byte lines), written for the copy in
-// parameters and moments, and in the moments for the source: some 56 lines a pair.  Measured: 300 pairs 5.6 + 6.7 us, 50 000
-// of a million Gaussians 19 + 39 us from the caches, 100 us from memory.
+// parameters and moments, and in the moments for the source: some 56 lines a pair.  Measured: 300 pairs 5.3 + 6.6 us, 50 000
+// of a million Gaussians 19 + 39 us from the caches; a call on rows that are not in them 100 us, where 56 lines a pair are 37 at
+// a copy's rate: a row's loads stand behind its pair's opacity and extent, the moments' zeros behind the loads.
 #include <math.h>
 
 #include "gs_device.h"

@@ -22,17 +22,19 @@
 //                        way, and one draw in eight of the tail's lands on another index
 //
 // Two forms, by the length of a row:
-//   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row)
+//   up to 8192 entries: one workgroup per row does everything, the entries in its registers (k_sample_row); with many draws
+//   several, each with the whole selection
 //   longer: the row is cut into chunks of 4096 over the whole chip, and a launch per step (k_long_*).  With top-k, rows
-//   whose candidates behind the first digit number 8192 or fewer are listed and go on as a short row does (k_long_list)
+//   whose candidates behind the first digit number 8192 or fewer are listed, if they have few draws, and go on as a short
+//   row does (k_long_list)
 //
-// Measured (kernels, MI355X): 28 entries 4.8 us; 28 rows of 8160 with top-p 14.4 us; 1 M opacities, 50 000 draws 21 us (max
-// 2.9, sums 8.3, scan 2.0, draws 7.8); 5 M opacities at a temperature with top-p, 250 000 draws 127 us (digits 27 + 20 + 10,
-// sums 23, draws 31, the rest 16); 64 rows of 131072 bfloat16 with top-k and top-p 60 us a call (first digit 10, lists 16,
-// the listed rows 20, the launches for others 3 .. 5 each).  The second word of a weight is some 10 % of a long row's time
-// (1 M 18 -> 20 us a call, 5 M 111 -> 116, 64 x 131072 float32 with top-p 70 -> 81).  A pass over 5 M entries at the memory's
-// rate is 5 us: the digits and sums of powers are bound by fp64 issue (75 instructions an entry, 9 us a pass
-// at the peak rate) and the fixed 8 to 10 us of a launch that picks a digit, reads a row from the caches and adds up a
+// Measured (kernels, MI355X): 28 entries 4.8 us; 28 rows of 8160 with top-p 14.4 us; 1 M opacities, 50 000 draws 22 us (max
+// 2.9, sums 8.3 .. 9.4, scan 2.0 .. 3.9, draws 8.0); 5 M opacities at a temperature with top-p, 250 000 draws 128 us (digits
+// 27 + 20 + 10, sums 24, draws 31, the rest 16); 64 rows of 131072 bfloat16 with top-k and top-p 60 us a call (first digit 9,
+// lists 17, the listed rows 20, the launches for others 2 .. 5 each).  The second word of a weight is 10 to 20 % of a long
+// row's time (calls: 1 M 18 -> 20 us, 5 M 111 -> 115 .. 120, 64 x 131072 float32 with top-p 70 -> 81).  A pass over 5 M entries
+// at the memory's rate is 5 us: the digits and sums of powers are bound by fp64 issue (80 instructions an entry, 10 us a pass
+// at the peak rate) and the fixed 6 to 9 us of a launch that picks a digit, reads a row from the caches and adds up a
 // histogram.
 #include <math.h>
 

@@ -105,7 +105,8 @@ class Trainer:
         self.strategy, self.max_gaussians, self.min_opacity = strategy, int(max_gaussians), float(min_opacity)
         self.source_temperature, self.source_top_p = float(source_temperature), float(source_top_p)
         # weight of the tile lists' balance loss (gs_tile_balance) in the step's loss, mean over the cameras like the
-        # image loss; its gradient joins the opacities' behind every backward
+        # image loss; its gradient joins the opacities' behind every backward.  train_step returns the image's loss; the
+        # balance term of its camera, weighted, is balance_out[0] (a batch's: balance[0][0] of its lanes, the last two)
         self.balance_weight = float(balance_weight)
         self.segmented, self._ckpt = segmented, cabi.Checkpoints()
         t = lambda a: torch.as_tensor(np.ascontiguousarray(a) if isinstance(a, np.ndarray) else a,
@@ -133,7 +134,7 @@ class Trainer:
         self.num_cameras = num_cameras
         self.num_downscales, self.resolution_schedule = num_downscales, resolution_schedule
         self.sh_degree_interval = sh_degree_interval
-        # re-sort the Gaussians along a 3-D Morton curve whenever a refinement rebuilds the tensors:
+        # re-sort the Gaussians along a 3-D Morton curve whenever a refinement by thresholds rebuilds the tensors:
         # neighbours in space become neighbours in memory (binning scatter and the per-Gaussian
         # kernels gain locality: +1..3 % per iteration at 1 M Gaussians)
         self.morton_order = morton_order
@@ -542,7 +543,7 @@ class Trainer:
 
     def train_step(self, cam, gt, background, degrees_to_use: int):
         """One iteration of opensplat.cpp:151-170 for this rank's camera of the batch.
-        Returns the device tensor {mainLoss, l1, ssim} of THIS camera (no host sync)."""
+        Returns the device tensor {mainLoss, l1, ssim} of THIS camera (no host sync), without the balance term."""
         if self.graph:
             return self._train_step_graph(cam, gt, background, degrees_to_use)
         rgb = self.render(cam, background, degrees_to_use)
