@@ -4,7 +4,7 @@
   csrc/libgsplat_torch.so  libtorch autograd operators on top of the C ABI, g++
 
 hipcc cross-compiles gfx950 without a GPU.  Both are rebuilt only when a source is newer than the
-library.  The built .so files are git-ignored but travel with the gpurun snapshot.
+library.  The built .so files stay beside their sources and are git-ignored.
 """
 from __future__ import annotations
 
