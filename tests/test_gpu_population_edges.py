@@ -265,3 +265,20 @@ def test_sample_many_draws_of_short_rows(shape):
     u = dev(rng.random((rows, draws), dtype=np.float32))
     # (the temperature as the call takes it: of five million draws, some lie closer to a border than 0.8 to its float32)
     check_sample(x, u, temperature=float(np.float32(0.8)), top_p=0.9)
+
+
+def test_sample_long_rows_on_two_streams_at_once():
+    rng = np.random.default_rng(8)
+    calls = []
+    for r, c, kw in ((3, 60_000, dict(top_p=0.9)), (2, 200_000, dict(top_k=20_000, top_p=0.7)), (1, 500_000, dict()),
+                     (4, 30_000, dict(top_k=100))):
+        calls.append((logits_of(rng, r, c, "f32"), dev(rng.random((r, 500), dtype=np.float32)), kw))
+    want = [cabi.sample(x, u, **kw) for x, u, kw in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for turn in range(6):
+        for k, (x, u, kw) in enumerate(calls):
+            with torch.cuda.stream(streams[(turn + k) % 2]):
+                got.append((k, cabi.sample(x, u, **kw)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(ids, want[k]) for k, ids in got)
